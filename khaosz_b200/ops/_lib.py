@@ -84,6 +84,12 @@ def _declare(lib):
         "kb_broadcast_bf16": ([P, P, P, I, I, I, LL, ctypes.c_uint, P], I),
         "kb_unit_reduce_bf16": ([P, P, P, I, I, LL, F, P, I, ctypes.c_uint, I, I, P], I),
         "kb_peer_barrier": ([P, I, I, I, ctypes.c_uint, I, P], I),
+        "kb_moe_route_fwd": ([P, I, L, P, P, I, P, I, I, I, I, I, I, I, I, F, P], I),
+        "kb_moe_route_bwd": ([P, I, L, P, P, P, I, P, I, I, I, I, I, F, P], I),
+        "kb_moe_plan": ([P, I, I, I, I, P, P, P, P, P, P, P], I),
+        "kb_moe_experts_fwd": ([P, L, P, I, P, P, P, P, P, L, L, P, L, L, P, L, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, P], I),
+        "kb_moe_experts_bwd": ([P, L, P, P, P, P, P, P, P, P, P, P, L, L, P, L, L, P, L, L, P, P, P, P, P, P, I, P, L, L, P, L, L, P, L, L,
+                                I, I, I, I, I, I, I, P], I),
         "kb_rmsnorm_bwd_static": ([P, P, P, P, P, P, P, I, I, P], I),
     }
     for name, (argtypes, restype) in sigs.items():

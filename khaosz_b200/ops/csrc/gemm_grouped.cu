@@ -1,0 +1,584 @@
+// Products of the routed experts on the 5th-generation tensor cores: GEMMs whose rows (or whose K dimension)
+// fall into segments, one per expert, that only the device knows.
+//
+//   GATE_UP   h = w * silu(X Wg^T) * (X Wu^T), rows of X grouped by expert; also writes both projections
+//   DOWN      Y = H Wd^T
+//   DHID      dH' = dY Wd, and from it dG, dU and each row's part of the routing weight's gradient
+//   DX        dX = dG Wg + dU Wu
+//   DW_DOWN   dWd[e] = dY[e]^T H[e]
+//   DW_GU     dWg[e] = dG[e]^T X[e], dWu[e] = dU[e]^T X[e]
+//
+// Structure as in gemm_bf16.cu: a persistent CTA per SM, warp 0 feeds a 4-stage ring by TMA, one thread of
+// warp 1 issues tcgen05.mma into two 128x256 fp32 accumulators, warps 2-5 run the epilogue of one tile while
+// the next one is computed.  The list of 128-row tiles (expert, first row, end row) lies in device memory, so
+// the host never learns the counts; a tile is never shared by two experts.  A tile's surplus rows are those of
+// the next expert, or of nobody: they are computed and not stored.  In GATE_UP the 256 columns of a tile are
+// 128 gate features and the same 128 up features, so SwiGLU, the routing weight and the rounding to bf16 happen
+// once, in the epilogue.  In the weight gradients K runs over an expert's rows in steps of 16, the alignment of
+// its segment, whose padding rows are zero.  All waits are bounded (common.cuh).
+#include "common.cuh"
+#include "kb_api.h"
+#include "moe.cuh"
+
+namespace kb {
+namespace grouped {
+
+enum Mode { GATE_UP = 0, DOWN = 1, DHID = 2, DX = 3, DW_DOWN = 4, DW_GU = 5 };
+
+constexpr int BM = KB_MOE_TILE_ROWS;
+constexpr int BN = 256;
+constexpr int BK = 64;
+constexpr int UMMA_K = 16;
+constexpr int STAGES = 4;
+constexpr int A_BYTES = BM * BK * 2;
+constexpr int B_BYTES = BN * BK * 2;
+constexpr int ATOM_BYTES = BK * 128;
+constexpr int SMEM_BYTES = STAGES * (A_BYTES + B_BYTES) + 256 + 1024;
+constexpr int NUM_THREADS = 192;
+static_assert(BM == 128 && KB_MOE_ROW_ALIGN == UMMA_K, "a segment begins on a K step");
+
+struct Params {
+  const int4* tiles;    // row modes: [0].x tiles, then (expert, first row, end row, 0)
+  const int* offsets;   // weight-gradient modes: [E + 1]
+  int E, num_m, num_n;  // weight-gradient modes: M tiles of one matrix; all: N tiles
+  int num_k;            // row modes: K blocks (DX: of one of the two halves)
+  int M, N;             // valid rows of a weight gradient; valid columns
+  __nv_bfloat16 *out0, *out1, *out2;
+  long ld0, ld1, stride0, stride1;  // pitch and (weight gradients) distance of the experts
+  const __nv_bfloat16 *g, *u;       // DHID: [rows, N]
+  const float* rw;                  // GATE_UP, DHID: routing weight of a row
+  float* part;                      // DHID: [rows, num_n]
+  int accumulate;                   // weight gradients: add to what is there
+  int* err;
+};
+
+struct Unit {
+  int e, row0, end;   // row modes
+  int m0, n0, mat;    // m0, mat: weight-gradient modes
+  int k0, klen;       // weight-gradient modes: first row and number of rows of the segment
+};
+
+template <int MODE>
+__device__ __forceinline__ Unit unit_of(const Params& p, int u) {
+  Unit r;
+  if constexpr (MODE < DW_DOWN) {
+    const int m = u / p.num_n;
+    const int4 t = __ldg(p.tiles + 1 + m);
+    r.e = t.x; r.row0 = t.y; r.end = t.z;
+    r.n0 = (u - m * p.num_n) * (MODE == GATE_UP ? BN / 2 : BN);
+    r.m0 = r.mat = r.k0 = r.klen = 0;
+  } else {
+    int x = u / p.num_n;
+    r.n0 = (u - x * p.num_n) * BN;
+    const int m = x % p.num_m;
+    x /= p.num_m;
+    r.m0 = m * BM;
+    if constexpr (MODE == DW_GU) { r.mat = x & 1; r.e = x >> 1; }
+    else { r.mat = 0; r.e = x; }
+    r.k0 = __ldg(p.offsets + r.e);
+    r.klen = __ldg(p.offsets + r.e + 1) - r.k0;
+    r.row0 = r.end = 0;
+  }
+  return r;
+}
+template <int MODE>
+__device__ __forceinline__ int unit_count(const Params& p) {
+  if constexpr (MODE < DW_DOWN) return __ldg(reinterpret_cast<const int*>(p.tiles)) * p.num_n;
+  else return p.E * (MODE == DW_GU ? 2 : 1) * p.num_m * p.num_n;
+}
+template <int MODE>
+__device__ __forceinline__ int k_blocks(const Params& p, const Unit& t) {
+  if constexpr (MODE < DX) return p.num_k;
+  else if constexpr (MODE == DX) return 2 * p.num_k;
+  else return (t.klen + BK - 1) / BK;
+}
+
+__device__ __forceinline__ uint4 pack8(const float* f) {
+  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+}
+__device__ __forceinline__ void unpack8(const uint4& v, float* f) {
+  const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
+  f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+}
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
+template <int MODE>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a2,
+               const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_b2, const Params p) {
+  constexpr bool A_MN = MODE >= DW_DOWN;
+  constexpr bool B_MN = MODE >= DHID;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * A_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sB + STAGES * B_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 4);
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int total = unit_count<MODE>(p);
+
+  if (warp == 0) {
+    // ------------------------------- TMA producer -------------------------------
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int un = blockIdx.x; un < total && ok; un += gridDim.x) {
+        const Unit t = unit_of<MODE>(p, un);
+        const int nk = k_blocks<MODE>(p, t);
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, p.err, KB_ERR_TIMEOUT_EMPTY)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(&full[s], A_BYTES + B_BYTES);
+          uint8_t* a = sA + s * A_BYTES;
+          uint8_t* b = sB + s * B_BYTES;
+          if constexpr (MODE == GATE_UP) {
+            tma_load_2d(a, &tmap_a, &full[s], kb * BK, t.row0);
+            tma_load_3d(b, &tmap_b, &full[s], kb * BK, t.n0, t.e);
+            tma_load_3d(b + B_BYTES / 2, &tmap_b2, &full[s], kb * BK, t.n0, t.e);
+          } else if constexpr (MODE == DOWN) {
+            tma_load_2d(a, &tmap_a, &full[s], kb * BK, t.row0);
+            tma_load_3d(b, &tmap_b, &full[s], kb * BK, t.n0, t.e);
+          } else if constexpr (MODE == DHID || MODE == DX) {
+            const bool second = MODE == DX && kb >= p.num_k;
+            const int k = (second ? kb - p.num_k : kb) * BK;
+            tma_load_2d(a, second ? &tmap_a2 : &tmap_a, &full[s], k, t.row0);
+#pragma unroll
+            for (int i = 0; i < BN / 64; ++i) tma_load_3d(b + i * ATOM_BYTES, second ? &tmap_b2 : &tmap_b, &full[s], t.n0 + i * 64, k, t.e);
+          } else {
+            const int k = t.k0 + kb * BK;
+#pragma unroll
+            for (int i = 0; i < BM / 64; ++i) tma_load_2d(a + i * ATOM_BYTES, t.mat ? &tmap_a2 : &tmap_a, &full[s], t.m0 + i * 64, k);
+#pragma unroll
+            for (int i = 0; i < BN / 64; ++i) tma_load_2d(b + i * ATOM_BYTES, &tmap_b, &full[s], t.n0 + i * 64, k);
+          }
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------- MMA issuer -------------------------------
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc(BM, BN, A_MN, B_MN);
+      int s = 0;
+      uint32_t ph = 0;
+      int acc = 0;
+      uint32_t aph = 0;
+      bool ok = true;
+      for (int un = blockIdx.x; un < total && ok; un += gridDim.x) {
+        Unit t;
+        if constexpr (MODE >= DW_DOWN) t = unit_of<MODE>(p, un);
+        const int nk = k_blocks<MODE>(p, t);
+        if (nk == 0) continue;  // an expert without rows: the epilogue writes zeros
+        if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, p.err, KB_ERR_TIMEOUT_TMEM_EMPTY)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_wait(&full[s], ph, abort_flag, p.err, KB_ERR_TIMEOUT_FULL)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(sA + s * A_BYTES);
+          const uint32_t b_addr = smem_u32(sB + s * B_BYTES);
+          // the rows behind a segment belong to the next expert: K ends with the segment
+          const int steps = MODE >= DW_DOWN ? min(BK, t.klen - kb * BK) / UMMA_K : BK / UMMA_K;
+#pragma unroll
+          for (int j = 0; j < BK / UMMA_K; ++j) {
+            if (j >= steps) break;
+            const uint64_t a_desc = A_MN ? umma_desc_mnmajor(a_addr, j * UMMA_K, ATOM_BYTES) : umma_desc_kmajor(a_addr, j * UMMA_K * 2);
+            const uint64_t b_desc = B_MN ? umma_desc_mnmajor(b_addr, j * UMMA_K, ATOM_BYTES) : umma_desc_kmajor(b_addr, j * UMMA_K * 2);
+            umma_f16(d_tmem, a_desc, b_desc, idesc, (kb || j) ? 1u : 0u);
+          }
+          umma_commit(&empty[s]);
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (!ok) break;
+        umma_commit(&tfull[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          aph ^= 1u;
+        }
+      }
+    }
+  } else {
+    // ------------------------------- epilogue -------------------------------
+    const int q = warp & 3;  // TMEM lane quarter this warp may read
+    const int row = q * 32 + lane;
+    int acc = 0;
+    uint32_t aph = 0;
+    for (int un = blockIdx.x; un < total; un += gridDim.x) {
+      const Unit t = unit_of<MODE>(p, un);
+      const bool any_k = k_blocks<MODE>(p, t) > 0;
+      float w = 0.f;
+      if constexpr (MODE == GATE_UP || MODE == DHID)
+        if (t.row0 + row < t.end) w = p.rw[t.row0 + row];
+      if (any_k && !mbar_wait(&tfull[acc], aph, abort_flag, p.err, KB_ERR_TIMEOUT_TMEM_FULL)) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+      if constexpr (MODE < DW_DOWN) {
+        if (t.row0 + q * 32 < t.end) {  // uniform in the warp
+          const bool live = t.row0 + row < t.end;
+          const size_t grow = t.row0 + row;
+          if constexpr (MODE == GATE_UP) {
+#pragma unroll 1
+            for (int c = 0; c < BN / 64; ++c) {
+              const int col = t.n0 + c * 32;
+              if (col >= p.N) break;
+              uint32_t vg[32], vu[32];
+              tmem_ld_32x32b_x32(t_row + c * 32, vg);
+              tmem_ld_32x32b_x32(t_row + BN / 2 + c * 32, vu);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float g[8], u[8], h[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                  g[x] = __uint_as_float(vg[i * 8 + x]);
+                  u[x] = __uint_as_float(vu[i * 8 + x]);
+                  h[x] = w * (g[x] * sigmoid(g[x])) * u[x];
+                }
+                if (live && col + i * 8 < p.N) {
+                  *reinterpret_cast<uint4*>(p.out2 + grow * p.ld0 + col + i * 8) = pack8(h);
+                  if (p.out0) {
+                    *reinterpret_cast<uint4*>(p.out0 + grow * p.ld0 + col + i * 8) = pack8(g);
+                    *reinterpret_cast<uint4*>(p.out1 + grow * p.ld0 + col + i * 8) = pack8(u);
+                  }
+                }
+              }
+            }
+          } else if constexpr (MODE == DHID) {
+            float dot = 0.f;
+#pragma unroll 1
+            for (int c = 0; c < BN / 32; ++c) {
+              const int col = t.n0 + c * 32;
+              if (col >= p.N) break;
+              uint4 vg[4], vu[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                vg[i] = vu[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (live && col + i * 8 < p.N) {
+                  vg[i] = *reinterpret_cast<const uint4*>(p.g + grow * p.ld0 + col + i * 8);
+                  vu[i] = *reinterpret_cast<const uint4*>(p.u + grow * p.ld0 + col + i * 8);
+                }
+              }
+              uint32_t v[32];
+              tmem_ld_32x32b_x32(t_row + c * 32, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float g[8], u[8], dg[8], du[8];
+                unpack8(vg[i], g);
+                unpack8(vu[i], u);
+                if (live && col + i * 8 < p.N) {
+#pragma unroll
+                  for (int x = 0; x < 8; ++x) {
+                    const float d = __uint_as_float(v[i * 8 + x]), s = sigmoid(g[x]), act = g[x] * s;
+                    dot += d * (act * u[x]);
+                    dg[x] = w * d * u[x] * (s + act * (1.f - s));
+                    du[x] = w * d * act;
+                  }
+                  *reinterpret_cast<uint4*>(p.out0 + grow * p.ld0 + col + i * 8) = pack8(dg);
+                  *reinterpret_cast<uint4*>(p.out1 + grow * p.ld0 + col + i * 8) = pack8(du);
+                }
+              }
+            }
+            if (live) p.part[grow * p.num_n + t.n0 / BN] = dot;
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < BN / 32; ++c) {
+              const int col = t.n0 + c * 32;
+              if (col >= p.N) break;
+              uint32_t v[32];
+              tmem_ld_32x32b_x32(t_row + c * 32, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (live && col + i * 8 < p.N)
+                  *reinterpret_cast<uint4*>(p.out0 + grow * p.ld0 + col + i * 8) = pack8(reinterpret_cast<const float*>(v + i * 8));
+            }
+          }
+        }
+      } else {
+        const int m = t.m0 + row;
+        __nv_bfloat16* o = t.mat ? p.out1 + t.e * p.stride1 + m * p.ld1 : p.out0 + t.e * p.stride0 + m * p.ld0;
+        if (any_k || !p.accumulate) {
+#pragma unroll 1
+          for (int c = 0; c < BN / 32; ++c) {
+            const int col = t.n0 + c * 32;
+            if (col >= p.N) break;
+            uint32_t v[32];
+            if (any_k) {
+              tmem_ld_32x32b_x32(t_row + c * 32, v);
+              tmem_ld_wait();
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (m >= p.M || col + i * 8 >= p.N) continue;
+              uint4* at = reinterpret_cast<uint4*>(o + col + i * 8);
+              float f[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(v[i * 8 + x]);
+              if (p.accumulate) {
+                float old[8];
+                unpack8(*at, old);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) f[x] += old[x];
+              }
+              *at = pack8(f);
+            }
+          }
+        }
+      }
+      if (any_k) {  // accumulator fully read: hand it back to the MMA warp
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          aph ^= 1u;
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+struct Weight {  // [E, rows, cols] bf16, unit inner stride
+  const void* p;
+  long ld, stride;
+};
+
+static int rows_map(CUtensorMap* m, const void* base, int rows, int cols, int box_rows) {
+  return make_tmap_2d(m, base, 2, rows, cols, (uint64_t)cols * 2, box_rows, BK, true) ? KB_STATUS_TMAP_ERROR : KB_STATUS_OK;
+}
+static int weight_map(CUtensorMap* m, const Weight& w, int E, int rows, int cols, int box_rows) {
+  const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)E};
+  const uint64_t strides[2] = {(uint64_t)w.ld * 2, (uint64_t)w.stride * 2};
+  const uint32_t box[3] = {BK, (uint32_t)box_rows, 1};
+  return make_tmap_3d(m, w.p, 2, dims, strides, box, true) ? KB_STATUS_TMAP_ERROR : KB_STATUS_OK;
+}
+
+template <int MODE>
+static int launch(const CUtensorMap& a, const CUtensorMap& a2, const CUtensorMap& b, const CUtensorMap& b2, const Params& p, int dev, int grid,
+                  cudaStream_t st) {
+  static bool set[64] = {false};  // the attribute is per device
+  if (!set[dev & 63]) {
+    if (cudaFuncSetAttribute(grouped_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return KB_STATUS_CUDA_ERROR;
+    set[dev & 63] = true;
+  }
+  grouped_kernel<MODE><<<grid, NUM_THREADS, SMEM_BYTES, st>>>(a, a2, b, b2, p);
+  return cudaGetLastError() == cudaSuccess ? KB_STATUS_OK : KB_STATUS_CUDA_ERROR;
+}
+
+static int cdiv(int a, int b) { return (a + b - 1) / b; }
+
+static bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool weight_ok(const Weight& w, int cols) { return w.p && aligned(w.p) && !(w.ld & 7) && !(w.stride & 7) && w.ld >= cols && w.stride > 0; }
+
+struct Device {
+  int dev = 0, sms = 0;
+  int* err = nullptr;
+};
+static int device(Device* d) {
+  static int sms[64] = {0};
+  if (cudaGetDevice(&d->dev) != cudaSuccess) return KB_STATUS_CUDA_ERROR;
+  int& n = sms[d->dev & 63];
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d->dev) != cudaSuccess) return KB_STATUS_CUDA_ERROR;
+  d->sms = n;
+  d->err = error_word(d->dev);
+  return KB_STATUS_OK;
+}
+
+}  // namespace grouped
+}  // namespace kb
+
+#define KB_TRY(x)                               \
+  do {                                          \
+    const int kb_rc = (x);                      \
+    if (kb_rc != KB_STATUS_OK) return kb_rc;    \
+  } while (0)
+
+// The sizes that both directions check: R grouped rows, at most `tiles` 128-row tiles of them.
+static int moe_sizes(int T, int k, int D, int F, int E, int R) {
+  if (T < 1 || k < 1 || D < 8 || F < 8 || E < 1 || R < 1 || (D & 7) || (F & 7)) return KB_STATUS_BAD_ARG;
+  if (E > KB_MOE_MAX_EXPERTS || (long long)T * k > (1 << 30)) return KB_STATUS_TOO_LARGE;
+  return KB_STATUS_OK;
+}
+
+extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, int w_f32, const int* offsets, const int* slots, const int* rows,
+                                  const int* tiles, const void* wg, long ldg, long sg, const void* wu, long ldu, long su, const void* wd, long ldd,
+                                  long sd, const void* res, long ldr, void* out, void* xs, float* rw, void* g, void* u, void* h, void* y, int T, int k,
+                                  int D, int F, int E, int R, void* stream) {
+  using namespace kb::grouped;
+  KB_TRY(moe_sizes(T, k, D, F, E, R));
+  const Weight G{wg, ldg, sg}, U{wu, ldu, su}, W{wd, ldd, sd};
+  if (!weight_ok(G, D) || !weight_ok(U, D) || !weight_ok(W, F) || !aligned(x) || (ldx & 7) || (res && (!aligned(res) || (ldr & 7)))) return KB_STATUS_BAD_ARG;
+  if (!aligned(out) || !aligned(xs) || !aligned(g) || !aligned(u) || !aligned(h) || !aligned(y) || !aligned(tiles) || (g == nullptr) != (u == nullptr))
+    return KB_STATUS_BAD_ARG;
+  Device d;
+  KB_TRY(device(&d));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  KB_TRY(kb::moe::launch_gather(x, ldx, rows, offsets + E, weights, w_f32, rw, xs, k, D, R, d.sms, st));
+  CUtensorMap a, b, b2;
+  Params p{};
+  p.tiles = reinterpret_cast<const int4*>(tiles);
+  p.offsets = offsets;
+  p.E = E;
+  p.err = d.err;
+  KB_TRY(rows_map(&a, xs, R, D, BM));
+  KB_TRY(weight_map(&b, G, E, F, D, BN / 2));
+  KB_TRY(weight_map(&b2, U, E, F, D, BN / 2));
+  p.num_n = cdiv(F, BN / 2);
+  p.num_k = cdiv(D, BK);
+  p.N = F;
+  p.out0 = static_cast<__nv_bfloat16*>(g);
+  p.out1 = static_cast<__nv_bfloat16*>(u);
+  p.out2 = static_cast<__nv_bfloat16*>(h);
+  p.ld0 = F;
+  p.rw = rw;
+  KB_TRY(launch<GATE_UP>(a, a, b, b2, p, d.dev, d.sms, st));
+  KB_TRY(rows_map(&a, h, R, F, BM));
+  KB_TRY(weight_map(&b, W, E, D, F, BN));
+  p.num_n = cdiv(D, BN);
+  p.num_k = cdiv(F, BK);
+  p.N = D;
+  p.out0 = static_cast<__nv_bfloat16*>(y);
+  p.out1 = p.out2 = nullptr;
+  p.ld0 = D;
+  KB_TRY(launch<DOWN>(a, a, b, b, p, d.dev, d.sms, st));
+  return kb::moe::launch_combine(y, slots, res, ldr, out, nullptr, 0, nullptr, 0, T, k, D, st);
+}
+
+extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, const float* rw, const void* g, const void* u, const void* h,
+                                  const int* offsets, const int* slots, const int* rows, const int* tiles, const void* wg, long ldg, long sg,
+                                  const void* wu, long ldu, long su, const void* wd, long ldd, long sd, void* dys, void* dg, void* du, float* part,
+                                  void* dx, void* dw, int w_f32, void* dwg, long ldwg, long sdwg, void* dwu, long ldwu, long sdwu, void* dwd, long ldwd,
+                                  long sdwd, int accumulate, int T, int k, int D, int F, int E, int R, void* stream) {
+  using namespace kb::grouped;
+  KB_TRY(moe_sizes(T, k, D, F, E, R));
+  const Weight G{wg, ldg, sg}, U{wu, ldu, su}, W{wd, ldd, sd};
+  if (!weight_ok(G, D) || !weight_ok(U, D) || !weight_ok(W, F) || !aligned(dout) || (ldo & 7) || (dwg == nullptr) != (dwu == nullptr)) return KB_STATUS_BAD_ARG;
+  if (dwg && (!weight_ok({dwg, ldwg, sdwg}, D) || !weight_ok({dwu, ldwu, sdwu}, D))) return KB_STATUS_BAD_ARG;
+  if (dwd && !weight_ok({dwd, ldwd, sdwd}, F)) return KB_STATUS_BAD_ARG;
+  if (!aligned(xs) || !aligned(g) || !aligned(u) || !aligned(h) || !aligned(dys) || !aligned(dg) || !aligned(du) || !aligned(dx) || !aligned(tiles))
+    return KB_STATUS_BAD_ARG;
+  Device d;
+  KB_TRY(device(&d));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  KB_TRY(kb::moe::launch_gather(dout, ldo, rows, offsets + E, nullptr, 0, nullptr, dys, k, D, R, d.sms, st));
+  CUtensorMap a, a2, b, b2;
+  Params p{};
+  p.tiles = reinterpret_cast<const int4*>(tiles);
+  p.offsets = offsets;
+  p.E = E;
+  p.err = d.err;
+  // dG, dU and the routing weights' partial gradients
+  const int n_part = cdiv(F, BN);
+  KB_TRY(rows_map(&a, dys, R, D, BM));
+  KB_TRY(weight_map(&b, W, E, D, F, BK));
+  p.num_n = n_part;
+  p.num_k = cdiv(D, BK);
+  p.N = F;
+  p.out0 = static_cast<__nv_bfloat16*>(dg);
+  p.out1 = static_cast<__nv_bfloat16*>(du);
+  p.ld0 = F;
+  p.g = static_cast<const __nv_bfloat16*>(g);
+  p.u = static_cast<const __nv_bfloat16*>(u);
+  p.rw = rw;
+  p.part = part;
+  KB_TRY(launch<DHID>(a, a, b, b, p, d.dev, d.sms, st));
+  p.g = p.u = nullptr;
+  p.part = nullptr;
+  p.accumulate = accumulate;
+  if (dwd) {  // before dX, which is written over dY's rows
+    KB_TRY(rows_map(&a, dys, R, D, BK));
+    KB_TRY(rows_map(&b, h, R, F, BK));
+    p.num_m = cdiv(D, BM);
+    p.num_n = cdiv(F, BN);
+    p.M = D;
+    p.N = F;
+    p.out0 = static_cast<__nv_bfloat16*>(dwd);
+    p.ld0 = ldwd;
+    p.stride0 = sdwd;
+    KB_TRY(launch<DW_DOWN>(a, a, b, b, p, d.dev, d.sms, st));
+  }
+  if (dx) {
+    KB_TRY(rows_map(&a, dg, R, F, BM));
+    KB_TRY(rows_map(&a2, du, R, F, BM));
+    KB_TRY(weight_map(&b, G, E, F, D, BK));
+    KB_TRY(weight_map(&b2, U, E, F, D, BK));
+    p.num_n = cdiv(D, BN);
+    p.num_k = cdiv(F, BK);
+    p.N = D;
+    p.out0 = static_cast<__nv_bfloat16*>(dys);
+    p.ld0 = D;
+    KB_TRY(launch<DX>(a, a2, b, b2, p, d.dev, d.sms, st));
+  }
+  if (dx || dw) KB_TRY(kb::moe::launch_combine(dys, slots, nullptr, 0, dx, part, n_part, dw, w_f32, T, k, D, st));
+  if (dwg) {
+    KB_TRY(rows_map(&a, dg, R, F, BK));
+    KB_TRY(rows_map(&a2, du, R, F, BK));
+    KB_TRY(rows_map(&b, xs, R, D, BK));
+    p.num_m = cdiv(F, BM);
+    p.num_n = cdiv(D, BN);
+    p.M = F;
+    p.N = D;
+    p.out0 = static_cast<__nv_bfloat16*>(dwg);
+    p.ld0 = ldwg;
+    p.stride0 = sdwg;
+    p.out1 = static_cast<__nv_bfloat16*>(dwu);
+    p.ld1 = ldwu;
+    p.stride1 = sdwu;
+    KB_TRY(launch<DW_GU>(a, a2, b, b, p, d.dev, d.sms, st));
+  }
+  return KB_STATUS_OK;
+}

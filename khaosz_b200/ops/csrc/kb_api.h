@@ -200,6 +200,36 @@ int kb_gemm_comm(const void* const* a_ptrs, const void* const* b_ptrs, void* c_l
                  unsigned int* ready, unsigned int ready_target, unsigned long long* trace, int exit_barrier, unsigned int* epoch_dev, unsigned int* calls_dev,
                  void* stream);
 
+// ---- sparse feed-forward layer (moe.cu, gemm_grouped.cu) ------------------------------
+#define KB_MOE_ROW_ALIGN 16      // an expert's segment of the grouped rows begins on a multiple of this
+#define KB_MOE_TILE_ROWS 128     // rows of a tile of the grouped products
+#define KB_MOE_MAX_EXPERTS 1024
+// Routing: weights [T,k] and experts [T,k] (int64) of logits [T,E] (bf16 or fp32, pitch ldz); bias [E] or NULL is added
+// for the selection only.  k <= 32, n_groups <= 32, group_top 1 or 2.
+int kb_moe_route_fwd(const void* z, int z_f32, long ldz, const float* bias, void* w, int w_f32, long long* ids, int T, int E, int k,
+                     int sigmoid, int renorm, int n_groups, int topk_groups, int group_top, float scale, void* stream);
+// dz [T,E] (dense, type of z) from dw [T,k] and the experts that the forward pass chose.
+int kb_moe_route_bwd(const void* z, int z_f32, long ldz, const float* bias, const long long* ids, const void* dw, int w_f32, void* dz,
+                     int T, int E, int k, int sigmoid, int renorm, float scale, void* stream);
+// Grouping of n assignments by expert.  counts [E], offsets [E+1], slots [n], rows [R], tiles [1 + tiles][4] (16-byte aligned,
+// R / 128 + min(E, n) tiles at most); R >= n + 15 min(E, n) rounded up to 16; hist [ceil(n / 4096), E] scratch (n > 4096).
+// An index outside 0..E-1 is dropped (slot -1).
+int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int* counts, int* offsets, int* slots, int* rows, int* tiles, int* hist,
+                void* stream);
+// out = res + the experts' products; the plan's arrays, the weights [E, F, D], [E, F, D], [E, D, F] (pitch, distance of the experts),
+// and scratch: xs [R,D], rw [R], h [R,F], y [R,D] (may be xs); g, u [R,F] (both or neither) keep the projections for the backward pass.
+int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, int w_f32, const int* offsets, const int* slots, const int* rows,
+                       const int* tiles, const void* wg, long ldg, long sg, const void* wu, long ldu, long su, const void* wd, long ldd, long sd,
+                       const void* res, long ldr, void* out, void* xs, float* rw, void* g, void* u, void* h, void* y, int T, int k, int D, int F,
+                       int E, int R, void* stream);
+// Backward pass: dx [T,D], dw [T,k] and the weights' gradients, each optional (dwg and dwu together); accumulate: the weights' gradients are
+// added to what is there.  Scratch: dys [R,D], dg, du [R,F], part [R, ceil(F / 256)].
+int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, const float* rw, const void* g, const void* u, const void* h,
+                       const int* offsets, const int* slots, const int* rows, const int* tiles, const void* wg, long ldg, long sg, const void* wu,
+                       long ldu, long su, const void* wd, long ldd, long sd, void* dys, void* dg, void* du, float* part, void* dx, void* dw,
+                       int w_f32, void* dwg, long ldwg, long sdwg, void* dwu, long ldwu, long sdwu, void* dwd, long ldwd, long sdwd,
+                       int accumulate, int T, int k, int D, int F, int E, int R, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

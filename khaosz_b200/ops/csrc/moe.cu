@@ -1,0 +1,600 @@
+// Sparse feed-forward layer: routing (forward, backward), grouping of the assignments by expert, the
+// gather / combine passes around the grouped GEMMs of gemm_grouped.cu, and the products of a few tokens.
+//
+//   assignment a = (token t, slot j), expert e = experts[t][j], weight w = weights[t][j]
+//   out[t] = residual[t] + sum_j  w * (silu(x[t] Wg[e]^T) * (x[t] Wu[e]^T)) Wd[e]^T
+//
+// Grouped rows: every expert owns a segment of consecutive rows, in the order of its assignments, that
+// begins on a multiple of 16 rows (one K step of the tensor cores, so that the weight gradients can stop
+// at a segment's end); the up to 15 rows behind a segment's last assignment are zero.
+#include "common.cuh"
+#include "kb_api.h"
+
+namespace kb {
+namespace moe {
+
+constexpr int ALIGN = KB_MOE_ROW_ALIGN;
+constexpr int TILE = KB_MOE_TILE_ROWS;
+constexpr unsigned FULL = 0xffffffffu;
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_f(float* p, float v) { *p = v; }
+__device__ __forceinline__ void from_f(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+__device__ __forceinline__ float load_f(const void* p, size_t i, int f32) {
+  return f32 ? static_cast<const float*>(p)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_f(void* p, size_t i, int f32, float v) {
+  if (f32) static_cast<float*>(p)[i] = v;
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16(v);
+}
+
+// ---------------------------------------------------------------------------------------
+// routing
+// ---------------------------------------------------------------------------------------
+// One warp per token; lane l holds the experts l, l + 32, ...  The k largest selection scores are taken in
+// k rounds of a warp-wide maximum over order-preserving integer keys (redux.sync), ties to the lowest index.
+// Key 0: not to be chosen (behind the last expert, outside the chosen groups, already taken).
+__device__ __forceinline__ uint32_t key_of(float v) {
+  const int b = __float_as_int(v + 0.f);  // -0 becomes +0
+  return b < 0 ? ~(uint32_t)b : (uint32_t)b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t key_of(double v) {
+  const long long b = __double_as_longlong(v + 0.0);
+  return b < 0 ? ~(uint64_t)b : (uint64_t)b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double value_of(uint64_t k) {
+  return __longlong_as_double((long long)(k & 0x8000000000000000ull ? k & 0x7fffffffffffffffull : ~k));
+}
+__device__ __forceinline__ uint32_t warp_max_key(uint32_t k) { return __reduce_max_sync(FULL, k); }
+__device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
+  const uint32_t hi = __reduce_max_sync(FULL, (uint32_t)(k >> 32));
+  const uint32_t lo = __reduce_max_sync(FULL, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  return (uint64_t)hi << 32 | lo;
+}
+
+struct RouteParams {
+  const void* z;          // [T, E] logits, pitch ldz
+  const float* bias;      // [E] or null
+  void* w;                // [T, k]
+  long long* ids;         // [T, k]
+  long ldz;
+  int T, E, k;
+  int sigmoid, renorm, n_groups, topk_groups, group_top;
+  int w_f32;
+  float scale;
+};
+
+// The selected experts' weights from their own logits; lane j < k holds slot j.  With renormalisation the
+// common factor e^m (m: the largest selected logit, for the sigmoid where it is negative) is taken out, so
+// that a row whose selected scores are all tiny keeps its ratios.  `dis`: no weight (disabled or no slot).
+__device__ __forceinline__ float slot_weight(float z, bool dis, bool sigmoid, bool renorm, float row_max, float row_sum, float* one_minus) {
+  *one_minus = 1.f;
+  if (!sigmoid && !renorm) return dis ? 0.f : __fdividef(__expf(z - row_max), row_sum);
+  float s;
+  float m = warp_max(dis ? -INFINITY : z);
+  if (sigmoid) {
+    m = renorm ? fminf(m, 0.f) : 0.f;
+    s = z > 0.f ? 1.f / (1.f + __expf(-z)) : __expf(z - m) / (1.f + __expf(z));
+    *one_minus = z > 0.f ? __expf(-z) / (1.f + __expf(-z)) : 1.f / (1.f + __expf(z));
+  } else {
+    s = __expf(z - m);
+  }
+  if (dis) s = 0.f;
+  if (!renorm) return s;
+  const float total = warp_sum(s);
+  return total > 0.f ? s / total : (total == 0.f ? 0.f : total);   // a NaN total stays one
+}
+
+template <int VPL, typename T, typename Key>
+__global__ void __launch_bounds__(256) route_fwd_kernel(const RouteParams p) {
+  const int lane = threadIdx.x & 31;
+  const int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (t >= p.T) return;
+  const T* zrow = static_cast<const T*>(p.z) + (size_t)t * p.ldz;
+  constexpr bool WIDE = sizeof(Key) == 8;
+  float z[VPL];
+  bool bad = false;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int e = i * 32 + lane;
+    z[i] = e < p.E ? to_f(zrow[e]) : -INFINITY;
+    bad |= isnan(z[i]) || (!p.sigmoid && z[i] == INFINITY);
+    m = fmaxf(m, z[i]);
+  }
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (i * 32 + lane < p.E) bad |= isnan(p.bias[i * 32 + lane]);
+  }
+  m = warp_max(m);
+  if (__any_sync(FULL, bad)) {  // no distribution: valid indices, weights that show it
+    if (lane < p.k) {
+      p.ids[(size_t)t * p.k + lane] = lane;
+      store_f(p.w, (size_t)t * p.k + lane, p.w_f32, NAN);
+    }
+    return;
+  }
+  // selection keys
+  Key key[VPL];
+  if constexpr (!WIDE) {  // the score is monotone in the logit
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) key[i] = i * 32 + lane < p.E ? key_of(z[i]) : 0u;
+  } else {
+    double s[VPL], total = 0.0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      if (p.sigmoid) {
+        s[i] = 1.0 / (1.0 + exp(-(double)z[i]));
+      } else {
+        s[i] = z[i] == -INFINITY ? 0.0 : exp((double)z[i] - (double)m);
+        total += s[i];
+      }
+    }
+    if (!p.sigmoid) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = i * 32 + lane;
+      if (e < p.E) {
+        double c = p.sigmoid ? s[i] : (total > 0.0 ? s[i] / total : 0.0);
+        if (p.bias) c += (double)p.bias[e];
+        key[i] = key_of(z[i] == -INFINITY ? -(double)INFINITY : c);
+      } else {
+        key[i] = 0;
+      }
+    }
+  }
+  if (p.n_groups > 1) {
+    const int gs = p.E / p.n_groups;
+    int grp[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) grp[i] = i * 32 + lane < p.E ? (i * 32 + lane) / gs : -1;
+    Key mine = 0;  // lane g: the key of group g
+    for (int g = 0; g < p.n_groups; ++g) {
+      Key best = 0;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (grp[i] == g && key[i] > best) best = key[i];
+      const Key top = warp_max_key(best);
+      Key score = top;
+      if constexpr (WIDE) {
+        if (p.group_top == 2 && gs > 1) {
+          // the second largest: one holder of the largest steps back
+          const unsigned who = __ballot_sync(FULL, best == top);
+          Key second = 0;
+          bool skipped = lane != __ffs(who) - 1;
+#pragma unroll
+          for (int i = 0; i < VPL; ++i) {
+            if (grp[i] != g) continue;
+            if (!skipped && key[i] == top) skipped = true;
+            else if (key[i] > second) second = key[i];
+          }
+          score = key_of(value_of(top) + value_of(warp_max_key(second)));
+        }
+      }
+      if (lane == g) mine = score;
+    }
+    unsigned keep = 0;
+    for (int r = 0; r < p.topk_groups; ++r) {
+      const Key top = warp_max_key(mine);
+      const int g = __ffs(__ballot_sync(FULL, mine == top)) - 1;
+      keep |= 1u << g;
+      if (lane == g) mine = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (grp[i] < 0 || !(keep >> grp[i] & 1u)) key[i] = 0;
+  }
+  int mine_e = 0;
+  for (int j = 0; j < p.k; ++j) {
+    Key best = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) best = key[i] > best ? key[i] : best;
+    const Key top = warp_max_key(best);
+    int at = p.E;
+#pragma unroll
+    for (int i = VPL - 1; i >= 0; --i)
+      if (key[i] == top) at = i * 32 + lane;
+    const int e = (int)__reduce_min_sync(FULL, (unsigned)at);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (e == i * 32 + lane) key[i] = 0;
+    if (lane == j) mine_e = e;
+  }
+  float row_sum = 1.f;
+  if (!p.sigmoid && !p.renorm) {
+    row_sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) row_sum += z[i] == -INFINITY ? 0.f : __expf(z[i] - m);
+    row_sum = warp_sum(row_sum);
+  }
+  const bool slot = lane < p.k;
+  const float zs = slot ? to_f(zrow[mine_e]) : -INFINITY;
+  const bool dis = !slot || zs == -INFINITY || (p.bias && p.bias[mine_e] == -INFINITY);
+  float om;
+  const float w = p.scale * slot_weight(zs, dis, p.sigmoid, p.renorm, m, row_sum, &om);
+  if (slot) {
+    p.ids[(size_t)t * p.k + lane] = mine_e;
+    store_f(p.w, (size_t)t * p.k + lane, p.w_f32, w);
+  }
+}
+
+// dz of one token (one warp): a sum over the selected slots, and for the softmax without renormalisation a
+// dense row.  Scores are recomputed from the logits in fp32.
+template <int VPL, typename T>
+__global__ void __launch_bounds__(256) route_bwd_kernel(const RouteParams p, const void* dw, T* dz) {
+  const int lane = threadIdx.x & 31;
+  const int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (t >= p.T) return;
+  const T* zrow = static_cast<const T*>(p.z) + (size_t)t * p.ldz;
+  const bool slot = lane < p.k;
+  const int e = slot ? (int)p.ids[(size_t)t * p.k + lane] : 0;
+  const float zs = slot ? to_f(zrow[e]) : -INFINITY;
+  const float g = slot ? load_f(dw, (size_t)t * p.k + lane, p.w_f32) : 0.f;
+  const bool dis = !slot || zs == -INFINITY || (p.bias && p.bias[e] == -INFINITY);
+  const bool dense = !p.sigmoid && !p.renorm;
+  float out[VPL];
+  float m = -INFINITY, row_sum = 1.f;
+  if (dense) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      out[i] = i * 32 + lane < p.E ? to_f(zrow[i * 32 + lane]) : -INFINITY;
+      m = isnan(out[i]) ? NAN : fmaxf(m, out[i]);
+    }
+    m = warp_max(m);
+    row_sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      out[i] = out[i] == -INFINITY ? 0.f : __expf(out[i] - m);
+      row_sum += out[i];
+    }
+    row_sum = warp_sum(row_sum);
+  }
+  float om;
+  const float w = slot_weight(zs, dis, p.sigmoid, p.renorm, m, row_sum, &om);
+  const float gd = dis ? 0.f : g;
+  const float mean = p.renorm || dense ? warp_sum(gd * w) : 0.f;
+  float d;  // this slot's own term
+  if (dense) d = p.scale * gd;
+  else d = p.scale * w * (p.sigmoid ? om : 1.f) * (gd - mean);
+  if (dis) d = 0.f;
+  const float inv = dense && row_sum > 0.f ? 1.f / row_sum : (row_sum == 0.f ? 0.f : row_sum);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) out[i] = dense ? out[i] * inv : 0.f;
+  float own[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) own[i] = 0.f;
+  for (int j = 0; j < p.k; ++j) {
+    const int ej = __shfl_sync(FULL, e, j);
+    const float dj = __shfl_sync(FULL, d, j);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (ej == i * 32 + lane) own[i] = dj;
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int c = i * 32 + lane;
+    if (c < p.E) from_f(dz + (size_t)t * p.E + c, dense ? out[i] * (own[i] - p.scale * mean) : own[i]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// grouping
+// ---------------------------------------------------------------------------------------
+// Stable counting sort without atomics on the result: a block owns CHUNK consecutive assignments, a warp 128
+// of them in four steps of 32; __match_any_sync ranks equal experts inside a step, per-warp counters in shared
+// memory carry the rank over the steps, a prefix over the warps and over the blocks completes it.
+constexpr int PLAN_THREADS = 1024;
+constexpr int STEPS = 4;
+constexpr int CHUNK = PLAN_THREADS * STEPS;
+
+struct PlanParams {
+  const void* ids;
+  int ids64, n, E, R, nb;
+  int* counts;    // [E]
+  int* offsets;   // [E + 1]
+  int* slots;     // [n]
+  int* rows;      // [R]
+  int4* tiles;    // [1 + max]: .x of the first = number of 128-row tiles, then (expert, first row, end row, 0)
+  int* hist;      // [nb, E] (several blocks only)
+};
+
+__device__ __forceinline__ int expert_of(const PlanParams& p, int a) {
+  if (a >= p.n) return -1;
+  const long long e = p.ids64 ? static_cast<const long long*>(p.ids)[a] : (long long)static_cast<const int*>(p.ids)[a];
+  return e < 0 || e >= p.E ? -1 : (int)e;
+}
+
+// Counts of each block's chunk; the rows are preset to "no assignment".
+__global__ void __launch_bounds__(PLAN_THREADS) plan_count_kernel(const PlanParams p) {
+  __shared__ int h[1024];
+  for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS) h[e] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int e = expert_of(p, blockIdx.x * CHUNK + s * PLAN_THREADS + threadIdx.x);
+    if (e >= 0) atomicAdd(&h[e], 1);
+  }
+  for (int r = blockIdx.x * PLAN_THREADS + threadIdx.x; r < p.R; r += gridDim.x * PLAN_THREADS) p.rows[r] = -1;
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS) p.hist[(size_t)blockIdx.x * p.E + e] = h[e];
+}
+
+// Exclusive prefix of two values per thread over the block.
+__device__ __forceinline__ void block_prefix2(int& a, int& b, int (*red)[2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = a, y = b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(FULL, x, o), v = __shfl_up_sync(FULL, y, o);
+    if (lane >= o) { x += u; y += v; }
+  }
+  if (lane == 31) { red[warp][0] = x; red[warp][1] = y; }
+  __syncthreads();
+  int bx = 0, by = 0;
+  for (int w = 0; w < warp; ++w) { bx += red[w][0]; by += red[w][1]; }
+  a = x - a + bx;
+  b = y - b + by;
+}
+
+// SINGLE: one block holds all assignments and nothing was counted before.
+template <bool SINGLE>
+__global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanParams p) {
+  extern __shared__ uint16_t wc[];  // [32 warps][E]
+  __shared__ int start[1024];       // first row of this block's assignments of an expert
+  __shared__ int red[32][2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint16_t* mine = wc + warp * p.E;
+  for (int e = lane; e < p.E; e += 32) mine[e] = 0;
+  if (SINGLE)
+    for (int r = tid; r < p.R; r += PLAN_THREADS) p.rows[r] = -1;
+  __syncwarp();
+  int ex[STEPS], rank[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) ex[s] = expert_of(p, blockIdx.x * CHUNK + warp * (32 * STEPS) + s * 32 + lane);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const unsigned same = __match_any_sync(FULL, ex[s]);
+    const int base = ex[s] >= 0 ? mine[ex[s]] : 0;
+    const int r = __popc(same & ((1u << lane) - 1u));
+    rank[s] = base + r;
+    __syncwarp();
+    if (ex[s] >= 0 && r == 0) mine[ex[s]] = (uint16_t)(base + __popc(same));
+    __syncwarp();
+  }
+  __syncthreads();
+  int in_block = 0;
+  if (tid < p.E) {
+#pragma unroll 8
+    for (int w = 0; w < 32; ++w) {
+      const int c = wc[w * p.E + tid];
+      wc[w * p.E + tid] = (uint16_t)in_block;
+      in_block += c;
+    }
+  }
+  int total = in_block, before = 0;
+  if (!SINGLE && tid < p.E) {
+    total = 0;
+#pragma unroll 8
+    for (int b = 0; b < p.nb; ++b) {
+      const int c = p.hist[(size_t)b * p.E + tid];
+      if (b < (int)blockIdx.x) before += c;
+      total += c;
+    }
+  }
+  if (tid >= p.E) total = 0;
+  const int padded = (total + ALIGN - 1) / ALIGN * ALIGN;
+  const int tiles = (padded + TILE - 1) / TILE;
+  int off = padded, first = tiles;
+  block_prefix2(off, first, red);
+  if (tid < p.E) start[tid] = off + before;
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    if (tid < p.E) {
+      p.counts[tid] = total;
+      p.offsets[tid] = off;
+      for (int i = 0; i < tiles; ++i) p.tiles[1 + first + i] = make_int4(tid, off + i * TILE, off + padded, 0);
+      if (tid == p.E - 1) {
+        p.offsets[p.E] = off + padded;
+        p.tiles[0] = make_int4(first + tiles, 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int a = blockIdx.x * CHUNK + warp * (32 * STEPS) + s * 32 + lane;
+    if (a >= p.n) continue;
+    const int e = ex[s];
+    const int r = e < 0 ? -1 : start[e] + wc[warp * p.E + e] + rank[s];
+    p.slots[a] = r;
+    if (e >= 0) p.rows[r] = a;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// passes around the products
+// ---------------------------------------------------------------------------------------
+// Grouped copy of token rows: dst[r] = src[rows[r] / k]; padding rows are zero.  One warp per row.
+// With `rw`: the row's routing weight too (0 for padding).
+__global__ void __launch_bounds__(256) gather_kernel(const __nv_bfloat16* src, long ld, const int* rows, const int* end, const void* w, int w_f32,
+                                                     float* rw, __nv_bfloat16* dst, int k, int D) {
+  const int lane = threadIdx.x & 31;
+  const int last = *end;
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < last; r += gridDim.x * 8) {
+    const int a = rows[r];
+    uint4* o = reinterpret_cast<uint4*>(dst + (size_t)r * D);
+    if (a < 0) {
+      for (int c = lane; c < D / 8; c += 32) o[c] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      const uint4* s = reinterpret_cast<const uint4*>(src + (size_t)(a / k) * ld);
+#pragma unroll 4
+      for (int c = lane; c < D / 8; c += 32) o[c] = s[c];
+    }
+    if (rw && lane == 0) rw[r] = a < 0 ? 0.f : load_f(w, a, w_f32);
+  }
+}
+
+// out[t] = residual[t] + sum_j y[slots[t][j]] in fp32, rounded once; a dropped slot adds nothing.
+// With `part`: dweights[t][j] = sum over the feature tiles of its row's partial dot products.
+__global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, const int* slots, const __nv_bfloat16* res, long ldr, __nv_bfloat16* out,
+                                                      const float* part, int n_part, void* dw, int w_f32, int T, int k, int D) {
+  const int per = D / 8;
+  const int lanes = per < 256 ? per : 256;  // threads that share a token
+  const int groups = 256 / lanes;
+  const int g = threadIdx.x / lanes, c0 = threadIdx.x % lanes;
+  if (g >= groups) return;
+  const int t = blockIdx.x * groups + g;
+  if (t >= T) return;
+  const int* sl = slots + (size_t)t * k;
+  if (out) {
+    for (int c = c0; c < per; c += lanes) {
+      float acc[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+      for (int j = 0; j < k; ++j) {
+        const int r = sl[j];
+        if (r < 0) continue;
+        const uint4 v = *reinterpret_cast<const uint4*>(y + (size_t)r * D + c * 8);
+        const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), d = unpack_bf16x2(v.z), f = unpack_bf16x2(v.w);
+        acc[0] += a.x; acc[1] += a.y; acc[2] += b.x; acc[3] += b.y;
+        acc[4] += d.x; acc[5] += d.y; acc[6] += f.x; acc[7] += f.y;
+      }
+      if (res) {
+        const uint4 v = *reinterpret_cast<const uint4*>(res + (size_t)t * ldr + c * 8);
+        const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), d = unpack_bf16x2(v.z), f = unpack_bf16x2(v.w);
+        acc[0] += a.x; acc[1] += a.y; acc[2] += b.x; acc[3] += b.y;
+        acc[4] += d.x; acc[5] += d.y; acc[6] += f.x; acc[7] += f.y;
+      }
+      *reinterpret_cast<uint4*>(out + (size_t)t * D + c * 8) =
+          make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]), pack_bf16x2(acc[6], acc[7]));
+    }
+  }
+  if (dw) {
+    for (int j = c0; j < k; j += lanes) {
+      float s = 0.f;
+      const int r = sl[j];
+      if (r >= 0)
+        for (int i = 0; i < n_part; ++i) s += part[(size_t)r * n_part + i];
+      store_f(dw, (size_t)t * k + j, w_f32, s);
+    }
+  }
+}
+
+}  // namespace moe
+}  // namespace kb
+
+// ---------------------------------------------------------------------------------------
+// C entries
+// ---------------------------------------------------------------------------------------
+namespace {
+using namespace kb::moe;
+
+inline int launched() { return cudaGetLastError() == cudaSuccess ? KB_STATUS_OK : KB_STATUS_CUDA_ERROR; }
+
+int route_check(const RouteParams& p) {
+  if (p.T < 0 || p.E < 1 || p.k < 1 || p.k > p.E || p.n_groups < 1 || p.topk_groups < 1 || p.topk_groups > p.n_groups) return KB_STATUS_BAD_ARG;
+  if (p.E % p.n_groups || (long)p.topk_groups * (p.E / p.n_groups) < p.k || p.group_top < 1 || p.group_top > 2) return KB_STATUS_BAD_ARG;
+  if (p.E > KB_MOE_MAX_EXPERTS || p.k > 32 || p.n_groups > 32) return KB_STATUS_TOO_LARGE;
+  return KB_STATUS_OK;
+}
+
+template <typename T, typename Key>
+void route_fwd(const RouteParams& p, cudaStream_t st) {
+  const int grid = (p.T + 7) / 8;
+  const int vpl = (p.E + 31) / 32;
+  if (vpl <= 1) route_fwd_kernel<1, T, Key><<<grid, 256, 0, st>>>(p);
+  else if (vpl <= 2) route_fwd_kernel<2, T, Key><<<grid, 256, 0, st>>>(p);
+  else if (vpl <= 4) route_fwd_kernel<4, T, Key><<<grid, 256, 0, st>>>(p);
+  else if (vpl <= 8) route_fwd_kernel<8, T, Key><<<grid, 256, 0, st>>>(p);
+  else if (vpl <= 16) route_fwd_kernel<16, T, Key><<<grid, 256, 0, st>>>(p);
+  else route_fwd_kernel<32, T, Key><<<grid, 256, 0, st>>>(p);
+}
+template <typename T>
+void route_bwd(const RouteParams& p, const void* dw, void* dz, cudaStream_t st) {
+  const int grid = (p.T + 7) / 8;
+  const int vpl = (p.E + 31) / 32;
+  T* o = static_cast<T*>(dz);
+  if (vpl <= 1) route_bwd_kernel<1, T><<<grid, 256, 0, st>>>(p, dw, o);
+  else if (vpl <= 2) route_bwd_kernel<2, T><<<grid, 256, 0, st>>>(p, dw, o);
+  else if (vpl <= 4) route_bwd_kernel<4, T><<<grid, 256, 0, st>>>(p, dw, o);
+  else if (vpl <= 8) route_bwd_kernel<8, T><<<grid, 256, 0, st>>>(p, dw, o);
+  else if (vpl <= 16) route_bwd_kernel<16, T><<<grid, 256, 0, st>>>(p, dw, o);
+  else route_bwd_kernel<32, T><<<grid, 256, 0, st>>>(p, dw, o);
+}
+}  // namespace
+
+extern "C" int kb_moe_route_fwd(const void* z, int z_f32, long ldz, const float* bias, void* w, int w_f32, long long* ids, int T, int E, int k,
+                                int sigmoid, int renorm, int n_groups, int topk_groups, int group_top, float scale, void* stream) {
+  RouteParams p{z, bias, w, ids, ldz, T, E, k, sigmoid, renorm, n_groups, topk_groups, group_top, w_f32, scale};
+  if (const int rc = route_check(p)) return rc;
+  if (T == 0) return KB_STATUS_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Without a bias and without sums of group scores the order of the scores is the order of the logits; else
+  // scores next to the border of the k largest need more than fp32 to be told apart.
+  const bool wide = bias != nullptr || (n_groups > 1 && group_top == 2 && E / n_groups > 1);
+  if (z_f32) wide ? route_fwd<float, uint64_t>(p, st) : route_fwd<float, uint32_t>(p, st);
+  else wide ? route_fwd<__nv_bfloat16, uint64_t>(p, st) : route_fwd<__nv_bfloat16, uint32_t>(p, st);
+  return launched();
+}
+
+extern "C" int kb_moe_route_bwd(const void* z, int z_f32, long ldz, const float* bias, const long long* ids, const void* dw, int w_f32, void* dz, int T,
+                                int E, int k, int sigmoid, int renorm, float scale, void* stream) {
+  RouteParams p{z, bias, nullptr, const_cast<long long*>(ids), ldz, T, E, k, sigmoid, renorm, 1, 1, 1, w_f32, scale};
+  if (const int rc = route_check(p)) return rc;
+  if (T == 0) return KB_STATUS_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (z_f32) route_bwd<float>(p, dw, dz, st);
+  else route_bwd<__nv_bfloat16>(p, dw, dz, st);
+  return launched();
+}
+
+extern "C" int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int* counts, int* offsets, int* slots, int* rows, int* tiles, int* hist,
+                           void* stream) {
+  if (n < 1 || E < 1) return KB_STATUS_BAD_ARG;
+  if (E > KB_MOE_MAX_EXPERTS || n > (1 << 30)) return KB_STATUS_TOO_LARGE;
+  const int least = (n + (ALIGN - 1) * (E < n ? E : n) + ALIGN - 1) / ALIGN * ALIGN;
+  if (R < least || (reinterpret_cast<uintptr_t>(tiles) & 15)) return KB_STATUS_BAD_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int nb = (n + CHUNK - 1) / CHUNK;
+  PlanParams p{ids, ids64, n, E, R, nb, counts, offsets, slots, rows, reinterpret_cast<int4*>(tiles), hist};
+  const int smem = 32 * E * 2;
+  if (nb == 1) {
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(plan_place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return KB_STATUS_CUDA_ERROR;
+    plan_place_kernel<true><<<1, PLAN_THREADS, smem, st>>>(p);
+  } else {
+    if (hist == nullptr) return KB_STATUS_BAD_ARG;
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(plan_place_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return KB_STATUS_CUDA_ERROR;
+    plan_count_kernel<<<nb, PLAN_THREADS, 0, st>>>(p);
+    plan_place_kernel<false><<<nb, PLAN_THREADS, smem, st>>>(p);
+  }
+  return launched();
+}
+
+namespace kb {
+namespace moe {
+
+// grouped copy of [T, D] rows (used by the forward and the backward pass of the products)
+int launch_gather(const void* src, long ld, const int* rows, const int* end, const void* w, int w_f32, float* rw, void* dst, int k, int D, int R, int sms,
+                  cudaStream_t st) {
+  const int want = (R + 7) / 8, cap = sms * 8;
+  gather_kernel<<<want < cap ? want : cap, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(src), ld, rows, end, w, w_f32, rw,
+                                                         static_cast<__nv_bfloat16*>(dst), k, D);
+  return launched();
+}
+
+int launch_combine(const void* y, const int* slots, const void* res, long ldr, void* out, const float* part, int n_part, void* dw, int w_f32, int T, int k,
+                   int D, cudaStream_t st) {
+  const int per = D / 8, lanes = per < 256 ? per : 256, groups = 256 / lanes;
+  combine_kernel<<<(T + groups - 1) / groups, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(y), slots, static_cast<const __nv_bfloat16*>(res), ldr,
+                                                            static_cast<__nv_bfloat16*>(out), part, n_part, dw, w_f32, T, k, D);
+  return launched();
+}
+
+}  // namespace moe
+}  // namespace kb

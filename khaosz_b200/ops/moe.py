@@ -1,0 +1,443 @@
+"""Operators of the sparse feed-forward layer.
+
+* :func:`moe_route` — routing: softmax or sigmoid scores, a selection bias for balance, limited groups of experts,
+  top-k, renormalised and scaled weights; the gradient reaches the logits.
+* :func:`moe_plan` — the assignments grouped by expert, on the device: counts, segments, and the row of every assignment.
+* :func:`moe_experts` — the experts' SwiGLU products and their weighted sum, forward and backward, as grouped tcgen05
+  GEMMs over the segments.  No count ever reaches the host, so a forward or a training step can be recorded as a CUDA graph.
+
+CUDA bf16 tensors (for the routing also fp32 logits) run on the kernels; everything else runs the plain PyTorch form,
+which is the oracle of the tests.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from ._lib import check, lib, stream
+from .functional import _count_use, _use_done
+
+ROW_ALIGN = 16      # an expert's segment of the grouped rows begins on a multiple of this
+TILE_ROWS = 128     # rows of one tile of the grouped products
+MAX_EXPERTS = 1024
+MAX_SLOTS = 32      # experts per token, and groups of experts
+PLAN_CHUNK = 4096   # assignments that one block of the grouping kernel takes
+
+Stack = Union[Tensor, Sequence[Tensor]]
+
+
+def _call(t: Tensor, name: str, *args) -> None:
+    """One entry of the kernel library on the current stream of ``t``'s device."""
+    if t.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(t.device):
+            return _call(t, name, *args)
+    check(getattr(lib(), name)(*args, stream()), name[3:])
+
+
+def _p(t: Optional[Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _round_up(n: int, to: int) -> int:
+    return (n + to - 1) // to * to
+
+
+# ---------------------------------------------------------------------------------------
+# routing
+# ---------------------------------------------------------------------------------------
+
+
+def _select(z: Tensor, bias: Optional[Tensor], k: int, sigmoid: bool, n_groups: int, topk_groups: int, group_top: int) -> Tensor:
+    z = z.detach().double()
+    if sigmoid:
+        s = torch.sigmoid(z)
+    else:
+        top = z.amax(-1, keepdim=True)
+        e = torch.exp(z - top.masked_fill(top == -torch.inf, 0.0))
+        total = e.sum(-1, keepdim=True)
+        s = e / total.masked_fill(total == 0, 1.0)
+    if bias is not None:
+        s = s + bias.detach().double()
+    s = s.masked_fill(z == -torch.inf, -torch.inf)
+    if n_groups > 1:
+        T, E = s.shape
+        g = s.view(T, n_groups, E // n_groups).sort(dim=-1, descending=True).values[..., :group_top].sum(-1)
+        best = g.sort(dim=-1, descending=True, stable=True).indices[:, :topk_groups]
+        keep = torch.zeros_like(g, dtype=torch.bool).scatter(1, best, True).repeat_interleave(E // n_groups, dim=1)
+        s = torch.where(keep, s.clamp(min=-1e300), torch.full_like(s, -torch.inf))
+    return s.sort(dim=-1, descending=True, stable=True).indices[:, :k]
+
+
+def _route_torch(z, bias, k, sigmoid, n_groups, topk_groups, group_top, renormalize, scale, dtype):
+    zf = z.float() if z.dtype != torch.float64 else z
+    bad = torch.isnan(zf) if sigmoid else torch.isnan(zf) | (zf == torch.inf)
+    if bias is not None:
+        bad = bad | torch.isnan(bias)
+    bad = bad.any(-1, keepdim=True)
+    ids = _select(torch.where(bad, torch.zeros_like(zf), zf), None if bias is None else bias.nan_to_num(nan=0.0, posinf=torch.inf, neginf=-torch.inf),
+                  k, sigmoid, n_groups, topk_groups, group_top)
+    ids = torch.where(bad, torch.arange(k, device=z.device), ids)
+    picked = zf.gather(1, ids)
+    off = picked == -torch.inf
+    if bias is not None:
+        off = off | (bias[ids] == -torch.inf)
+    if not sigmoid and not renormalize:
+        top = zf.detach().amax(-1, keepdim=True)
+        e = torch.exp(zf - top.masked_fill(top == -torch.inf, 0.0))
+        total = e.sum(-1, keepdim=True)
+        w = (e / total.masked_fill(total == 0, 1.0)).gather(1, ids)
+    elif sigmoid:
+        w = torch.sigmoid(picked)
+    else:
+        top = picked.detach().masked_fill(off, -torch.inf).amax(-1, keepdim=True)
+        w = torch.exp(picked.masked_fill(off, -torch.inf) - top.masked_fill(top == -torch.inf, 0.0))
+    w = w.masked_fill(off, 0.0)
+    if renormalize:
+        total = w.sum(-1, keepdim=True)
+        w = w / total.masked_fill(total == 0, 1.0)
+    w = torch.where(bad, torch.full_like(w, torch.nan), w * scale)
+    return w.to(dtype), ids
+
+
+class _RouteFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, bias, k, sigmoid, n_groups, topk_groups, group_top, renormalize, scale, dtype):
+        T, E = z.shape
+        w = torch.empty((T, k), dtype=dtype, device=z.device)
+        ids = torch.empty((T, k), dtype=torch.long, device=z.device)
+        f32, w32 = int(z.dtype == torch.float32), int(dtype == torch.float32)
+        _call(z, "kb_moe_route_fwd", _p(z), f32, z.stride(0), _p(bias), _p(w), w32, _p(ids), T, E, k, int(sigmoid), int(renormalize), n_groups,
+              topk_groups, group_top, scale)
+        ctx.save_for_backward(z, bias, ids)
+        ctx.args = (k, int(sigmoid), int(renormalize), scale, f32, w32)
+        ctx.mark_non_differentiable(ids)
+        return w, ids
+
+    @staticmethod
+    def backward(ctx, dw, _):
+        z, bias, ids = ctx.saved_tensors
+        k, sigmoid, renormalize, scale, f32, w32 = ctx.args
+        T, E = z.shape
+        dw = dw.contiguous()
+        dz = torch.empty((T, E), dtype=z.dtype, device=z.device)
+        _call(z, "kb_moe_route_bwd", _p(z), f32, z.stride(0), _p(bias), _p(ids), _p(dw), w32, _p(dz), T, E, k, sigmoid, renormalize, scale)
+        return (dz,) + (None,) * 9
+
+
+def moe_route(logits: Tensor, k: int, *, score: str = "softmax", bias: Optional[Tensor] = None, n_groups: int = 1, topk_groups: int = 1,
+              group_top: int = 2, renormalize: bool = True, scale: float = 1.0, dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
+    """The ``k`` experts of every token and their weights: ``(weights [..., k], experts [..., k] int64)`` of ``logits [..., E]``.
+
+    The scores are ``softmax(logits)`` or ``sigmoid(logits)``.  Experts are chosen by score plus ``bias`` (``[E]``, it takes no
+    gradient and leaves the weights alone), in descending order, ties to the lowest index.  With ``n_groups > 1`` the experts
+    form that many groups of neighbours and only those of the ``topk_groups`` best groups can be chosen; a group counts the sum of
+    its ``group_top`` (1 or 2) largest selection scores.  The weights are the chosen experts' scores, divided by their sum with
+    ``renormalize``, times ``scale``, in ``dtype`` (default: that of the logits).
+
+    A logit or a bias of minus infinity disables an expert: it is chosen only where no other is left and has weight 0, so a row
+    of nothing else has weights 0.  A row with a NaN (for the softmax also with plus infinity) has weights NaN and the experts
+    ``0..k-1``.  Supports up to 1024 experts, 32 groups and ``k <= 32``.
+    """
+    if logits.dim() < 1 or not logits.is_floating_point():
+        raise ValueError("moe_route: logits must be a floating-point tensor [..., experts]")
+    E = logits.shape[-1]
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"moe_route: unknown score {score!r} (softmax or sigmoid)")
+    if not 1 <= k <= min(E, MAX_SLOTS) or E > MAX_EXPERTS:
+        raise ValueError(f"moe_route: k={k} of {E} experts (1 <= k <= min(experts, {MAX_SLOTS}), at most {MAX_EXPERTS} experts)")
+    if not 1 <= n_groups <= MAX_SLOTS or E % n_groups or not 1 <= topk_groups <= n_groups or group_top not in (1, 2):
+        raise ValueError(f"moe_route: {E} experts in {n_groups} groups, {topk_groups} of them taken by their {group_top} largest scores")
+    if topk_groups * (E // n_groups) < k:
+        raise ValueError(f"moe_route: {topk_groups} groups of {E // n_groups} experts hold fewer than k={k}")
+    if bias is not None and (bias.shape != (E,) or not bias.is_floating_point() or bias.device != logits.device):
+        raise ValueError("moe_route: bias must be a floating-point tensor [experts] on the logits' device")
+    dtype = logits.dtype if dtype is None else dtype
+    lead = logits.shape[:-1]
+    z = logits.reshape(-1, E)
+    args = (int(k), score == "sigmoid", int(n_groups), int(topk_groups), int(group_top), bool(renormalize), float(scale), dtype)
+    if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32) or dtype not in (torch.bfloat16, torch.float32):
+        w, ids = _route_torch(z, bias, *args)
+    else:
+        if z.stride(-1) != 1 and E > 1 or z.stride(0) < E:
+            z = z.contiguous()
+        w, ids = _RouteFn.apply(z, None if bias is None else bias.detach().float().contiguous(), *args)
+    return w.view(*lead, k), ids.view(*lead, k)
+
+
+# ---------------------------------------------------------------------------------------
+# grouping
+# ---------------------------------------------------------------------------------------
+
+
+class MoEPlan(NamedTuple):
+    """Assignments grouped by expert (all int32, on the experts' device).
+
+    ``counts [E]``; ``offsets [E + 1]``: first row of each expert's segment (a multiple of 16), last entry: the end; ``slots``
+    (shape of the experts): the row of each assignment, -1 where it is dropped; ``rows``: the assignment ``t * k + j`` of each
+    row, -1 where it has none; ``tiles``: entry 0 holds the number of 128-row tiles, then ``(expert, first row, end row, 0)``."""
+
+    counts: Tensor
+    offsets: Tensor
+    slots: Tensor
+    rows: Tensor
+    tiles: Tensor
+
+
+def rows_bound(n: int, n_experts: int) -> int:
+    """Rows that hold ``n`` assignments to ``n_experts`` experts in any case."""
+    return _round_up(n + (ROW_ALIGN - 1) * min(n, n_experts), ROW_ALIGN)
+
+
+def _tiles_bound(n: int, n_experts: int) -> int:
+    return rows_bound(n, n_experts) // TILE_ROWS + min(n, n_experts)
+
+
+def _check_ids(experts: Tensor, n_experts: int, who: str) -> None:
+    if experts.dtype not in (torch.int64, torch.int32) or experts.dim() < 1:
+        raise ValueError(f"{who}: experts must be an int64 or int32 tensor [..., k]")
+    if not 1 <= n_experts <= MAX_EXPERTS:
+        raise ValueError(f"{who}: {n_experts} experts (1 to {MAX_EXPERTS})")
+    if experts.numel() > 1 << 30:
+        raise ValueError(f"{who}: more than 2^30 assignments")
+
+
+def _plan_torch(ids: Tensor, E: int) -> MoEPlan:
+    flat = ids.reshape(-1).long()
+    n, dev = flat.numel(), flat.device
+    live = (flat >= 0) & (flat < E)
+    key = torch.where(live, flat, torch.full_like(flat, E))
+    counts = torch.bincount(key, minlength=E + 1)[:E]
+    padded = (counts + ROW_ALIGN - 1) // ROW_ALIGN * ROW_ALIGN
+    offsets = torch.cat([padded.new_zeros(1), padded.cumsum(0)])
+    order = torch.argsort(key, stable=True)[: int(live.sum())]
+    of = key[order]
+    row = offsets[of] + torch.arange(order.numel(), device=dev) - (counts.cumsum(0) - counts)[of]
+    slots = torch.full_like(flat, -1)
+    slots[order] = row
+    rows = torch.full((rows_bound(n, E),), -1, dtype=torch.long, device=dev)
+    rows[row] = order
+    per = (padded + TILE_ROWS - 1) // TILE_ROWS
+    ex = torch.repeat_interleave(torch.arange(E, device=dev), per)
+    first = offsets[ex] + (torch.arange(ex.numel(), device=dev) - (per.cumsum(0) - per)[ex]) * TILE_ROWS
+    tiles = torch.zeros(1 + _tiles_bound(n, E), 4, dtype=torch.long, device=dev)
+    tiles[0, 0] = ex.numel()
+    tiles[1:1 + ex.numel()] = torch.stack([ex, first, offsets[ex + 1], torch.zeros_like(ex)], 1)
+    return MoEPlan(*(v.to(torch.int32) for v in (counts, offsets, slots.view(ids.shape), rows, tiles)))
+
+
+def moe_plan(experts: Tensor, n_experts: int) -> MoEPlan:
+    """Group the assignments ``experts [..., k]`` by expert, in their order (see :class:`MoEPlan`).  An index outside
+    ``0..n_experts-1`` is dropped: it takes no row (padded tokens carry -1).  Deterministic."""
+    _check_ids(experts, n_experts, "moe_plan")
+    n, E = experts.numel(), int(n_experts)
+    if not experts.is_cuda or n == 0:
+        return _plan_torch(experts, E)
+    ids = experts.contiguous()
+    R, blocks = rows_bound(n, E), -(-n // PLAN_CHUNK)
+    # tiles come first: they are read as 16-byte entries
+    sizes = [4 * (1 + _tiles_bound(n, E)), E, E + 1, n, R] + ([blocks * E] if blocks > 1 else [])
+    parts = torch.empty(sum(sizes), dtype=torch.int32, device=ids.device).split(sizes)
+    tiles, counts, offsets, slots, rows = parts[:5]
+    _call(ids, "kb_moe_plan", _p(ids), int(ids.dtype == torch.int64), n, E, R, _p(counts), _p(offsets), _p(slots), _p(rows), _p(tiles),
+          _p(parts[5]) if blocks > 1 else None)
+    if blocks > 1:
+        _lib.add_launches(1)
+    return MoEPlan(counts, offsets, slots.view(experts.shape), rows, tiles.view(-1, 4))
+
+
+# ---------------------------------------------------------------------------------------
+# experts' products
+# ---------------------------------------------------------------------------------------
+
+
+def _uniform(ws: Sequence[Tensor]) -> Optional[Tensor]:
+    """The ``[E, rows, cols]`` view over equally spaced matrices of one storage, if they are that."""
+    first = ws[0]
+    base, size = first.untyped_storage().data_ptr(), first.element_size()
+    at = first.data_ptr()
+    step = ws[1].data_ptr() - at if len(ws) > 1 else first.numel() * size
+    if step < first.numel() * size or step % size:
+        return None
+    for w in ws:
+        if w.data_ptr() != at or w.shape != first.shape or w.dtype != first.dtype or not w.is_contiguous() or w.untyped_storage().data_ptr() != base:
+            return None
+        at += step
+    return first.detach().as_strided((len(ws), *first.shape), (step // size, first.shape[1], 1), first.storage_offset())
+
+
+def _kernel_view(w: Tensor) -> Tensor:
+    """``w [E, rows, cols]`` as the kernels read it: unit inner stride, pitch and distance in multiples of 16 bytes."""
+    E, _, cols = w.shape
+    if (w.stride(2) != 1 or w.stride(1) < cols or w.stride(1) % 8 or w.data_ptr() % 16
+            or (E > 1 and (w.stride(0) < cols or w.stride(0) % 8))):
+        return w.contiguous()
+    return w
+
+
+def _stride0(w: Tensor) -> int:
+    return w.stride(0) if w.shape[0] > 1 else w.shape[1] * w.stride(1)
+
+
+def _stacked(group: Sequence[Tensor]) -> Tensor:
+    """One ``[E, rows, cols]`` tensor of a group: itself, a view over equally spaced experts, or a copy."""
+    if len(group) == 1 and group[0].dim() == 3:
+        return _kernel_view(group[0].detach())
+    view = _uniform(group)
+    return _kernel_view(view if view is not None else torch.stack([w.detach() for w in group]))
+
+
+def _grad_view(group: Sequence[Tensor]) -> Optional[Tensor]:
+    """The ``main_grad`` buffers of a group as one kernel-readable view, where they are that."""
+    mains = [getattr(w, "main_grad", None) for w in group]
+    if any(m is None or m.dtype != torch.bfloat16 for m in mains):
+        return None
+    view = mains[0] if len(group) == 1 and mains[0].dim() == 3 else _uniform(mains)
+    return view if view is not None and _kernel_view(view) is view else None
+
+
+class _Space:
+    """One allocation for the scratch of a pass; pieces are 16-byte aligned addresses into it."""
+
+    def __init__(self, device, **sizes: int):
+        at, self.offset = 0, {}
+        for name, nbytes in sizes.items():
+            self.offset[name] = at
+            at += _round_up(nbytes, 256)
+        self.buf = torch.empty(max(at, 1), dtype=torch.uint8, device=device)
+
+    def __getitem__(self, name: str):
+        return self.buf.data_ptr() + self.offset[name] if name in self.offset else None
+
+
+class _ExpertsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weights, residual, plan, n_each, train, *ws):
+        groups = [ws[i * n_each:(i + 1) * n_each] for i in range(3)]
+        wg, wu, wd = (_stacked(g) for g in groups)
+        (T, D), k, E, F = x.shape, weights.shape[1], wg.shape[0], wg.shape[1]
+        R = plan.rows.numel()
+        wide, hidden = 2 * R * D, 2 * R * F
+        sp = _Space(x.device, xs=wide, rw=4 * R, h=hidden, **(dict(g=hidden, u=hidden) if train else {}))
+        out = torch.empty((T, D), dtype=x.dtype, device=x.device)
+        # without a backward pass nobody reads the grouped inputs again: the products overwrite them
+        ybuf = torch.empty(wide, dtype=torch.uint8, device=x.device) if train else None
+        y = ybuf.data_ptr() if train else sp["xs"]
+        _call(x, "kb_moe_experts_fwd", _p(x), x.stride(0), _p(weights), int(weights.dtype == torch.float32), _p(plan.offsets), _p(plan.slots),
+              _p(plan.rows), _p(plan.tiles), _p(wg), wg.stride(1), _stride0(wg), _p(wu), wu.stride(1), _stride0(wu), _p(wd), wd.stride(1), _stride0(wd),
+              _p(residual), residual.stride(0) if residual is not None else 0, _p(out), sp["xs"], sp["rw"], sp["g"], sp["u"], sp["h"], y, T, k, D, F, E, R)
+        _lib.add_launches(3)
+        if train:
+            ctx.save_for_backward(sp.buf, wg, wu, wd, *plan)
+            ctx.space, ctx.groups = sp.offset, groups
+            ctx.sizes = (T, k, D, F, E, R, weights.dtype, n_each)
+            for i, w in enumerate(ws):
+                if ctx.needs_input_grad[6 + i]:
+                    _count_use(w)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        buf, wg, wu, wd, _, offsets, slots, rows, tiles = ctx.saved_tensors
+        T, k, D, F, E, R, w_dtype, n_each = ctx.sizes
+        at = {name: buf.data_ptr() + o for name, o in ctx.space.items()}
+        dout = _rows2d(dout)
+        dev = dout.device
+        need = ctx.needs_input_grad
+        n_part = -(-F // 256)
+        sp = _Space(dev, dys=2 * R * D, dg=2 * R * F, du=2 * R * F, part=4 * R * n_part)
+        dx = torch.empty((T, D), dtype=dout.dtype, device=dev) if need[0] else None
+        dw = torch.empty((T, k), dtype=w_dtype, device=dev) if need[1] else None
+        wants = [any(need[6 + i * n_each:6 + (i + 1) * n_each]) for i in range(3)]
+        mains = [_grad_view(g) for g in ctx.groups]
+        into = all(need[6:]) and all(m is not None for m in mains)
+        if into:
+            grads = mains
+        else:
+            both = wants[0] or wants[1]
+            grads = [torch.empty((E, F, D), dtype=wg.dtype, device=dev) if both else None,
+                     torch.empty((E, F, D), dtype=wg.dtype, device=dev) if both else None,
+                     torch.empty((E, D, F), dtype=wg.dtype, device=dev) if wants[2] else None]
+        where = [v for g in grads for v in ((_p(g), g.stride(1), _stride0(g)) if g is not None else (None, 0, 0))]
+        _call(dout, "kb_moe_experts_bwd", _p(dout), dout.stride(0), at["xs"], at["rw"], at["g"], at["u"], at["h"], _p(offsets), _p(slots), _p(rows),
+              _p(tiles), _p(wg), wg.stride(1), _stride0(wg), _p(wu), wu.stride(1), _stride0(wu), _p(wd), wd.stride(1), _stride0(wd), sp["dys"], sp["dg"],
+              sp["du"], sp["part"], _p(dx), _p(dw), int(w_dtype == torch.float32), *where, int(into), T, k, D, F, E, R)
+        _lib.add_launches(1 + bool(grads[2] is not None) + bool(need[0]) + bool(need[0] or need[1]) + bool(grads[0] is not None))
+        out = []
+        for i, group in enumerate(ctx.groups):
+            if into:
+                for w in group:
+                    w.main_grad_dirty = True
+                    _use_done(w)
+                out += [None] * n_each
+            else:
+                for j in range(n_each):
+                    wanted = need[6 + i * n_each + j]
+                    out.append((grads[i] if group[0].dim() == 3 else grads[i][j]) if wanted else None)
+        return (dx, dw, dout if need[2] else None, None, None, None, *out)
+
+
+def _rows2d(t: Tensor) -> Tensor:
+    """``[rows, D]`` with unit inner stride and a pitch in multiples of 16 bytes."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else t.contiguous()
+
+
+def _experts_torch(x, weights, ids, wg, wu, wd, residual):
+    dt = torch.float64 if x.dtype == torch.float64 else torch.float32
+    xf, out = x.to(dt), torch.zeros(x.shape, dtype=dt, device=x.device)
+    for e in range(len(wg)):
+        t, j = (ids == e).nonzero(as_tuple=True)
+        if t.numel():
+            rows = xf[t]
+            g = rows @ wg[e].to(dt).t()
+            h = g * torch.sigmoid(g) * (rows @ wu[e].to(dt).t()) * weights[t, j].to(dt).unsqueeze(1)
+            out = out.index_add(0, t, h @ wd[e].to(dt).t())
+    return (out if residual is None else out + residual.to(dt)).to(x.dtype)
+
+
+def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up: Stack, w_down: Stack, residual: Optional[Tensor] = None,
+                plan: Optional[MoEPlan] = None) -> Tensor:
+    """``residual + sum_j weights[..., j] * down(silu(gate(x)) * up(x))`` over each token's experts.
+
+    ``x [..., D]``; ``weights``, ``experts [..., k]`` as :func:`moe_route` gives them; ``w_gate``, ``w_up [E, F, D]`` and
+    ``w_down [E, D, F]`` as stacked tensors or as sequences of the experts' matrices (equally spaced ones, as flat parameter
+    buffers hold them, are read in place).  An index outside ``0..E-1`` is dropped.  ``plan``: the :func:`moe_plan` of these
+    experts, where it is at hand.  Gradients reach ``x``, ``weights``, ``residual`` and the experts' matrices, whose
+    ``main_grad`` buffers receive them in place; an expert without tokens gets zeros.
+
+    The kernels take CUDA bf16 with D and F in multiples of 8 (weights also fp32); sums are held in fp32 and rounded once,
+    the hidden activations and each expert's output row are bf16.
+    """
+    stacks = [[w] if isinstance(w, Tensor) else list(w) for w in (w_gate, w_up, w_down)]
+    n_each = len(stacks[0])
+    lone = isinstance(w_gate, Tensor)
+    shapes = [tuple(w.shape) if lone else (len(s), *s[0].shape) for s, w in zip(stacks, (w_gate, w_up, w_down)) if s]
+    if (len(shapes) < 3 or any(isinstance(w, Tensor) != lone for w in (w_gate, w_up, w_down)) or any(len(s) != 3 for s in shapes)
+            or shapes[1] != shapes[0] or shapes[2] != (shapes[0][0], shapes[0][2], shapes[0][1])
+            or any(w.shape != s[0].shape for s in stacks for w in s)):
+        raise ValueError(f"moe_experts: weights must be gate and up [E, F, D] and down [E, D, F], got {shapes}")
+    E, F, D = shapes[0]
+    _check_ids(experts, E, "moe_experts")
+    if x.dim() < 1 or x.shape[-1] != D or experts.shape[:-1] != x.shape[:-1] or weights.shape != experts.shape:
+        raise ValueError(f"moe_experts: x {tuple(x.shape)}, weights {tuple(weights.shape)}, experts {tuple(experts.shape)} do not fit [..., {D}], [..., k], [..., k]")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"moe_experts: residual {tuple(residual.shape)} has not the shape of x {tuple(x.shape)}")
+    k = experts.shape[-1]
+    every = [w for s in stacks for w in s]
+    if any(t.device != x.device for t in (weights, experts, *every, *([residual] if residual is not None else []))):
+        raise ValueError("moe_experts: all tensors must be on one device")
+    if plan is not None and (plan.slots.shape != experts.shape or plan.counts.numel() != E or plan.rows.device != x.device):
+        raise ValueError("moe_experts: the plan is not one of these experts")
+    x2, w2, ids2 = x.reshape(-1, D), weights.reshape(-1, k), experts.reshape(-1, k)
+    r2 = None if residual is None else residual.reshape(-1, D)
+    kernel = (x.is_cuda and x.dtype == torch.bfloat16 and all(w.dtype == torch.bfloat16 for w in every) and D % 8 == 0 and F % 8 == 0
+              and weights.dtype in (torch.bfloat16, torch.float32) and (r2 is None or r2.dtype == torch.bfloat16) and ids2.numel() > 0)
+    if not kernel:
+        return _experts_torch(x2, w2, ids2, *(s[0] if lone else s for s in stacks), r2).view(x.shape)
+    plan = moe_plan(ids2, E) if plan is None else plan
+    train = torch.is_grad_enabled() and any(t.requires_grad for t in (x2, w2, *every, *([r2] if r2 is not None else [])))
+    return _ExpertsFn.apply(_rows2d(x2), w2.contiguous(), None if r2 is None else _rows2d(r2), plan, n_each, train, *every).view(x.shape)
