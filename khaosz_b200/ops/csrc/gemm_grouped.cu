@@ -34,7 +34,8 @@ constexpr int A_BYTES = BM * BK * 2;
 constexpr int B_BYTES = BN * BK * 2;
 constexpr int ATOM_BYTES = BK * 128;
 constexpr int SMEM_BYTES = STAGES * (A_BYTES + B_BYTES) + 256 + 1024;
-constexpr int NUM_THREADS = 192;
+constexpr int EPI_WARPS = 8;  // two per TMEM lane quarter, each half of the columns
+constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
 static_assert(BM == 128 && KB_MOE_ROW_ALIGN == UMMA_K, "a segment begins on a K step");
 
 struct Params {
@@ -47,7 +48,7 @@ struct Params {
   long ld0, ld1, stride0, stride1;  // pitch and (weight gradients) distance of the experts
   const __nv_bfloat16 *g, *u;       // DHID: [rows, N]
   const float* rw;                  // GATE_UP, DHID: routing weight of a row
-  float* part;                      // DHID: [rows, num_n]
+  float* part;                      // DHID: [rows, 2 num_n]
   int accumulate;                   // weight gradients: add to what is there
   int* err;
 };
@@ -93,6 +94,12 @@ __device__ __forceinline__ int k_blocks(const Params& p, const Unit& t) {
   else return (t.klen + BK - 1) / BK;
 }
 
+// Columns of a tile that are computed: the last tile of a row stops at a multiple of 64.
+template <int MODE>
+__device__ __forceinline__ int tile_cols(const Params& p, const Unit& t) {
+  return MODE == GATE_UP ? BN : min(BN, (p.N - t.n0 + 63) / 64 * 64);
+}
+
 __device__ __forceinline__ uint4 pack8(const float* f) {
   return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
@@ -129,7 +136,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 4);
+      mbar_init(&tempty[i], EPI_WARPS);
     }
     mbar_fence_init();
     tma_prefetch_desc(&tmap_a);
@@ -143,6 +150,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  kb::moe::await_predecessor();
   const int total = unit_count<MODE>(p);
 
   if (warp == 0) {
@@ -154,12 +162,14 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       for (int un = blockIdx.x; un < total && ok; un += gridDim.x) {
         const Unit t = unit_of<MODE>(p, un);
         const int nk = k_blocks<MODE>(p, t);
+        const int atoms = tile_cols<MODE>(p, t) / 64;
+        const uint32_t bytes = A_BYTES + (B_MN ? atoms * ATOM_BYTES : B_BYTES);
         for (int kb = 0; kb < nk; ++kb) {
           if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, p.err, KB_ERR_TIMEOUT_EMPTY)) {
             ok = false;
             break;
           }
-          mbar_expect_tx(&full[s], A_BYTES + B_BYTES);
+          mbar_expect_tx(&full[s], bytes);
           uint8_t* a = sA + s * A_BYTES;
           uint8_t* b = sB + s * B_BYTES;
           if constexpr (MODE == GATE_UP) {
@@ -173,14 +183,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             const bool second = MODE == DX && kb >= p.num_k;
             const int k = (second ? kb - p.num_k : kb) * BK;
             tma_load_2d(a, second ? &tmap_a2 : &tmap_a, &full[s], k, t.row0);
-#pragma unroll
-            for (int i = 0; i < BN / 64; ++i) tma_load_3d(b + i * ATOM_BYTES, second ? &tmap_b2 : &tmap_b, &full[s], t.n0 + i * 64, k, t.e);
+            for (int i = 0; i < atoms; ++i) tma_load_3d(b + i * ATOM_BYTES, second ? &tmap_b2 : &tmap_b, &full[s], t.n0 + i * 64, k, t.e);
           } else {
             const int k = t.k0 + kb * BK;
 #pragma unroll
             for (int i = 0; i < BM / 64; ++i) tma_load_2d(a + i * ATOM_BYTES, t.mat ? &tmap_a2 : &tmap_a, &full[s], t.m0 + i * 64, k);
-#pragma unroll
-            for (int i = 0; i < BN / 64; ++i) tma_load_2d(b + i * ATOM_BYTES, &tmap_b, &full[s], t.n0 + i * 64, k);
+            for (int i = 0; i < atoms; ++i) tma_load_2d(b + i * ATOM_BYTES, &tmap_b, &full[s], t.n0 + i * 64, k);
           }
           if (++s == STAGES) {
             s = 0;
@@ -192,16 +200,17 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   } else if (warp == 1) {
     // ------------------------------- MMA issuer -------------------------------
     if (lane == 0) {
-      constexpr uint32_t idesc = umma_idesc(BM, BN, A_MN, B_MN);
       int s = 0;
       uint32_t ph = 0;
       int acc = 0;
       uint32_t aph = 0;
       bool ok = true;
       for (int un = blockIdx.x; un < total && ok; un += gridDim.x) {
-        Unit t;
+        Unit t{};
         if constexpr (MODE >= DW_DOWN) t = unit_of<MODE>(p, un);
+        else t.n0 = un % p.num_n * (MODE == GATE_UP ? BN / 2 : BN);
         const int nk = k_blocks<MODE>(p, t);
+        const uint32_t idesc = umma_idesc(BM, tile_cols<MODE>(p, t), A_MN, B_MN);
         if (nk == 0) continue;  // an expert without rows: the epilogue writes zeros
         if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, p.err, KB_ERR_TIMEOUT_TMEM_EMPTY)) {
           ok = false;
@@ -243,6 +252,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   } else {
     // ------------------------------- epilogue -------------------------------
     const int q = warp & 3;  // TMEM lane quarter this warp may read
+    const int half = (warp - 2) >> 2;
     const int row = q * 32 + lane;
     int acc = 0;
     uint32_t aph = 0;
@@ -261,7 +271,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           const size_t grow = t.row0 + row;
           if constexpr (MODE == GATE_UP) {
 #pragma unroll 1
-            for (int c = 0; c < BN / 64; ++c) {
+            for (int c = half * (BN / 128); c < (half + 1) * (BN / 128); ++c) {
               const int col = t.n0 + c * 32;
               if (col >= p.N) break;
               uint32_t vg[32], vu[32];
@@ -289,7 +299,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           } else if constexpr (MODE == DHID) {
             float dot = 0.f;
 #pragma unroll 1
-            for (int c = 0; c < BN / 32; ++c) {
+            for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
               const int col = t.n0 + c * 32;
               if (col >= p.N) break;
               uint4 vg[4], vu[4];
@@ -322,10 +332,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                 }
               }
             }
-            if (live) p.part[grow * p.num_n + t.n0 / BN] = dot;
+            if (live) p.part[(grow * p.num_n + t.n0 / BN) * 2 + half] = dot;
           } else {
 #pragma unroll 1
-            for (int c = 0; c < BN / 32; ++c) {
+            for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
               const int col = t.n0 + c * 32;
               if (col >= p.N) break;
               uint32_t v[32];
@@ -343,7 +353,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         __nv_bfloat16* o = t.mat ? p.out1 + t.e * p.stride1 + m * p.ld1 : p.out0 + t.e * p.stride0 + m * p.ld0;
         if (any_k || !p.accumulate) {
 #pragma unroll 1
-          for (int c = 0; c < BN / 32; ++c) {
+          for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
             const int col = t.n0 + c * 32;
             if (col >= p.N) break;
             uint32_t v[32];
@@ -415,8 +425,8 @@ static int launch(const CUtensorMap& a, const CUtensorMap& a2, const CUtensorMap
     if (cudaFuncSetAttribute(grouped_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return KB_STATUS_CUDA_ERROR;
     set[dev & 63] = true;
   }
-  grouped_kernel<MODE><<<grid, NUM_THREADS, SMEM_BYTES, st>>>(a, a2, b, b2, p);
-  return cudaGetLastError() == cudaSuccess ? KB_STATUS_OK : KB_STATUS_CUDA_ERROR;
+  return kb::moe::launch_after(grouped_kernel<MODE>, grid, NUM_THREADS, SMEM_BYTES, st, a, a2, b, b2, p) == cudaSuccess ? KB_STATUS_OK
+                                                                                                                         : KB_STATUS_CUDA_ERROR;
 }
 
 static int cdiv(int a, int b) { return (a + b - 1) / b; }
@@ -522,10 +532,10 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
   p.E = E;
   p.err = d.err;
   // dG, dU and the routing weights' partial gradients
-  const int n_part = cdiv(F, BN);
+  const int n_part = 2 * cdiv(F, BN);
   KB_TRY(rows_map(&a, dys, R, D, BM));
   KB_TRY(weight_map(&b, W, E, D, F, BK));
-  p.num_n = n_part;
+  p.num_n = cdiv(F, BN);
   p.num_k = cdiv(D, BK);
   p.N = F;
   p.out0 = static_cast<__nv_bfloat16*>(dg);

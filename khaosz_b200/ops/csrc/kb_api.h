@@ -204,6 +204,7 @@ int kb_gemm_comm(const void* const* a_ptrs, const void* const* b_ptrs, void* c_l
 #define KB_MOE_ROW_ALIGN 16      // an expert's segment of the grouped rows begins on a multiple of this
 #define KB_MOE_TILE_ROWS 128     // rows of a tile of the grouped products
 #define KB_MOE_MAX_EXPERTS 1024
+#define KB_MOE_SMALL_MAX 32      // assignments that the small form takes
 // Routing: weights [T,k] and experts [T,k] (int64) of logits [T,E] (bf16 or fp32, pitch ldz); bias [E] or NULL is added
 // for the selection only.  k <= 32, n_groups <= 32, group_top 1 or 2.
 int kb_moe_route_fwd(const void* z, int z_f32, long ldz, const float* bias, void* w, int w_f32, long long* ids, int T, int E, int k,
@@ -222,8 +223,12 @@ int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, int w_f32, 
                        const int* tiles, const void* wg, long ldg, long sg, const void* wu, long ldu, long su, const void* wd, long ldd, long sd,
                        const void* res, long ldr, void* out, void* xs, float* rw, void* g, void* u, void* h, void* y, int T, int k, int D, int F,
                        int E, int R, void* stream);
+// The same product for T * k <= KB_MOE_SMALL_MAX assignments, straight from the experts' indices (no plan); h [T*k, F] fp32 scratch.
+int kb_moe_experts_small(const void* x, long ldx, const void* weights, int w_f32, const void* ids, int ids64, const void* wg, long ldg, long sg,
+                         const void* wu, long ldu, long su, const void* wd, long ldd, long sd, const void* res, long ldr, void* out, float* h,
+                         int T, int k, int D, int F, int E, void* stream);
 // Backward pass: dx [T,D], dw [T,k] and the weights' gradients, each optional (dwg and dwu together); accumulate: the weights' gradients are
-// added to what is there.  Scratch: dys [R,D], dg, du [R,F], part [R, ceil(F / 256)].
+// added to what is there.  Scratch: dys [R,D], dg, du [R,F], part [R, 2 ceil(F / 256)].
 int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, const float* rw, const void* g, const void* u, const void* h,
                        const int* offsets, const int* slots, const int* rows, const int* tiles, const void* wg, long ldg, long sg, const void* wu,
                        long ldu, long su, const void* wd, long ldd, long sd, void* dys, void* dg, void* du, float* part, void* dx, void* dw,

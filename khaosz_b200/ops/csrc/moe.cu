@@ -9,6 +9,7 @@
 // at a segment's end); the up to 15 rows behind a segment's last assignment are zero.
 #include "common.cuh"
 #include "kb_api.h"
+#include "moe.cuh"
 
 namespace kb {
 namespace moe {
@@ -35,10 +36,17 @@ __device__ __forceinline__ void store_f(void* p, size_t i, int f32, float v) {
 // One warp per token; lane l holds the experts l, l + 32, ...  The k largest selection scores are taken in
 // k rounds of a warp-wide maximum over order-preserving integer keys (redux.sync), ties to the lowest index.
 // Key 0: not to be chosen (behind the last expert, outside the chosen groups, already taken).
+//
+// Which order is right.  Without a bias the order of the scores is the order of the logits, and the keys are
+// the logits themselves.  With a bias, or where groups are ranked by sums, scores next to a border can be
+// closer than fp32 tells apart: the keys are fp32 scores, and a row in which two neighbours in the ranking are
+// within the error of fp32 (and do not come from equal logits and biases, an exact tie) is ranked again in
+// fp64, about one row in a thousand.  All rows in fp64 took 176 us for 32768 tokens and 256 experts.
 __device__ __forceinline__ uint32_t key_of(float v) {
   const int b = __float_as_int(v + 0.f);  // -0 becomes +0
   return b < 0 ? ~(uint32_t)b : (uint32_t)b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(uint32_t k) { return __int_as_float((int)(k & 0x80000000u ? k & 0x7fffffffu : ~k)); }
 __device__ __forceinline__ uint64_t key_of(double v) {
   const long long b = __double_as_longlong(v + 0.0);
   return b < 0 ? ~(uint64_t)b : (uint64_t)b | 0x8000000000000000ull;
@@ -65,6 +73,124 @@ struct RouteParams {
   float scale;
 };
 
+// What an fp32 score may be off: below 5e-7 for either kind (1/(1+e^-z): 0.25 of e's error of at most 2^-21,
+// 0.22 * 2^-22 for the rounded argument, 2^-22 for the division, 2^-24 for the sum; e/sum likewise), and half
+// a step for adding the bias.  Two scores further apart than this are in the right order.
+__device__ __forceinline__ float near_score(float c) { return 2e-6f + fabsf(c) * 2.4e-7f; }
+
+// The groups that may be chosen from, as bits; `close`: the last one taken and the first one left are nearer
+// than `slack` times the error of a score.  WIDE keys are exact.
+template <int VPL, typename Key>
+__device__ __forceinline__ unsigned best_groups(const Key (&key)[VPL], const RouteParams& p, int lane, bool& close) {
+  constexpr bool EXACT = sizeof(Key) == 8;
+  const int gs = p.E / p.n_groups;
+  const bool two = p.group_top == 2 && gs > 1;
+  Key mine = 0;  // lane g: the key of group g
+  for (int g = 0; g < p.n_groups; ++g) {
+    const int lo = g * gs, hi = lo + gs;
+    Key best = 0, next = 0;  // this lane's two largest of the group
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = i * 32 + lane;
+      if (i * 32 + 31 < lo || i * 32 >= hi) continue;  // uniform
+      const Key k = e >= lo && e < hi ? key[i] : Key(0);
+      if (k > best) { next = best; best = k; }
+      else if (k > next) next = k;
+    }
+    const Key top = warp_max_key(best);
+    Key score = top;
+    if (two) {  // one holder of the largest steps back
+      if (lane == __ffs(__ballot_sync(FULL, best == top)) - 1) best = next;
+      score = key_of(value_of(top) + value_of(warp_max_key(best)));
+    }
+    if (lane == g) mine = score;
+  }
+  unsigned keep = 0;
+  Key last = 0;
+  for (int r = 0; r < p.topk_groups; ++r) {
+    last = warp_max_key(mine);
+    const int g = __ffs(__ballot_sync(FULL, mine == last)) - 1;
+    keep |= 1u << g;
+    if (lane == g) mine = 0;
+  }
+  if (!EXACT && p.topk_groups < p.n_groups) {
+    const float a = (float)value_of(last), b = (float)value_of(warp_max_key(mine));
+    close |= !(a - b > 2.f * near_score(a));
+  }
+  return keep;
+}
+
+// Lane j < k ends with the j-th expert in descending order of the keys.  `close` as above, for neighbours.
+template <int VPL, typename Key, typename T, bool TOLD>
+__device__ __forceinline__ int take_best(Key (&key)[VPL], const RouteParams& p, const T* zrow, int lane, bool& close) {
+  int mine = 0, prev_e = 0;
+  float prev = 0.f;
+  const int rounds = TOLD && p.k < p.E ? p.k + 1 : p.k;  // the first one left behind counts too
+  for (int j = 0; j < rounds; ++j) {
+    Key best = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) best = key[i] > best ? key[i] : best;
+    const Key top = warp_max_key(best);
+    if (TOLD && top == 0) break;  // nothing is left to be chosen
+    int at = p.E;
+#pragma unroll
+    for (int i = VPL - 1; i >= 0; --i)
+      if (key[i] == top) at = i * 32 + lane;
+    const int e = (int)__reduce_min_sync(FULL, (unsigned)at);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (e == i * 32 + lane) key[i] = 0;
+    if (lane == j) mine = e;
+    if constexpr (TOLD) {
+      const float c = (float)value_of(top);
+      if (j && !(prev - c > near_score(prev)) && c != -INFINITY)
+        close |= !(to_f(zrow[e]) == to_f(zrow[prev_e]) && (!p.bias || p.bias[e] == p.bias[prev_e]));
+      prev = c;
+      prev_e = e;
+    }
+  }
+  return mine;
+}
+
+template <int VPL, typename Key>
+__device__ __forceinline__ void only_groups(Key (&key)[VPL], const RouteParams& p, int lane, unsigned keep) {
+  const int gs = p.E / p.n_groups;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int e = i * 32 + lane;
+    if (e >= p.E || !(keep >> (e / gs) & 1u)) key[i] = 0;
+  }
+}
+
+// The whole ranking in fp64.
+template <int VPL, typename T>
+__device__ __noinline__ int rank_wide(const RouteParams& p, const T* zrow, int lane, float m) {
+  uint64_t key[VPL];
+  double total = 0.0;
+  if (!p.sigmoid) {
+    for (int e = lane; e < p.E; e += 32) {
+      const float z = to_f(zrow[e]);
+      total += z == -INFINITY ? 0.0 : exp((double)z - (double)m);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int e = i * 32 + lane;
+    key[i] = 0;
+    if (e < p.E) {
+      const float z = to_f(zrow[e]);
+      double c = -(double)INFINITY;
+      if (z != -INFINITY) c = (p.sigmoid ? 1.0 / (1.0 + exp(-(double)z)) : exp((double)z - (double)m) / total) + (p.bias ? (double)p.bias[e] : 0.0);
+      key[i] = key_of(c);
+    }
+  }
+  bool close = false;
+  if (p.n_groups > 1) only_groups(key, p, lane, best_groups(key, p, lane, close));
+  return take_best<VPL, uint64_t, T, false>(key, p, zrow, lane, close);
+}
+
 // The selected experts' weights from their own logits; lane j < k holds slot j.  With renormalisation the
 // common factor e^m (m: the largest selected logit, for the sigmoid where it is negative) is taken out, so
 // that a row whose selected scores are all tiny keeps its ratios.  `dis`: no weight (disabled or no slot).
@@ -86,13 +212,13 @@ __device__ __forceinline__ float slot_weight(float z, bool dis, bool sigmoid, bo
   return total > 0.f ? s / total : (total == 0.f ? 0.f : total);   // a NaN total stays one
 }
 
-template <int VPL, typename T, typename Key>
+// SCORED: the ranking needs the scores (a bias, or groups ranked by sums).
+template <int VPL, typename T, bool SCORED>
 __global__ void __launch_bounds__(256) route_fwd_kernel(const RouteParams p) {
   const int lane = threadIdx.x & 31;
   const int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (t >= p.T) return;
   const T* zrow = static_cast<const T*>(p.z) + (size_t)t * p.ldz;
-  constexpr bool WIDE = sizeof(Key) == 8;
   float z[VPL];
   bool bad = false;
   float m = -INFINITY;
@@ -103,12 +229,15 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(const RouteParams p) {
     bad |= isnan(z[i]) || (!p.sigmoid && z[i] == INFINITY);
     m = fmaxf(m, z[i]);
   }
-  if (p.bias) {
+  float b[VPL];
+  if constexpr (SCORED) {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (i * 32 + lane < p.E) bad |= isnan(p.bias[i * 32 + lane]);
+    for (int i = 0; i < VPL; ++i) {
+      b[i] = p.bias && i * 32 + lane < p.E ? __ldg(p.bias + i * 32 + lane) : 0.f;
+      bad |= isnan(b[i]);
+    }
   }
-  m = warp_max(m);
+  if (!p.sigmoid) m = warp_max(m);
   if (__any_sync(FULL, bad)) {  // no distribution: valid indices, weights that show it
     if (lane < p.k) {
       p.ids[(size_t)t * p.k + lane] = lane;
@@ -116,169 +245,110 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(const RouteParams p) {
     }
     return;
   }
-  // selection keys
-  Key key[VPL];
-  if constexpr (!WIDE) {  // the score is monotone in the logit
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) key[i] = i * 32 + lane < p.E ? key_of(z[i]) : 0u;
-  } else {
-    double s[VPL], total = 0.0;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      if (p.sigmoid) {
-        s[i] = 1.0 / (1.0 + exp(-(double)z[i]));
-      } else {
-        s[i] = z[i] == -INFINITY ? 0.0 : exp((double)z[i] - (double)m);
-        total += s[i];
-      }
-    }
-    if (!p.sigmoid) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
-    }
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = i * 32 + lane;
-      if (e < p.E) {
-        double c = p.sigmoid ? s[i] : (total > 0.0 ? s[i] / total : 0.0);
-        if (p.bias) c += (double)p.bias[e];
-        key[i] = key_of(z[i] == -INFINITY ? -(double)INFINITY : c);
-      } else {
-        key[i] = 0;
-      }
-    }
-  }
-  if (p.n_groups > 1) {
-    const int gs = p.E / p.n_groups;
-    int grp[VPL];
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) grp[i] = i * 32 + lane < p.E ? (i * 32 + lane) / gs : -1;
-    Key mine = 0;  // lane g: the key of group g
-    for (int g = 0; g < p.n_groups; ++g) {
-      Key best = 0;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (grp[i] == g && key[i] > best) best = key[i];
-      const Key top = warp_max_key(best);
-      Key score = top;
-      if constexpr (WIDE) {
-        if (p.group_top == 2 && gs > 1) {
-          // the second largest: one holder of the largest steps back
-          const unsigned who = __ballot_sync(FULL, best == top);
-          Key second = 0;
-          bool skipped = lane != __ffs(who) - 1;
-#pragma unroll
-          for (int i = 0; i < VPL; ++i) {
-            if (grp[i] != g) continue;
-            if (!skipped && key[i] == top) skipped = true;
-            else if (key[i] > second) second = key[i];
-          }
-          score = key_of(value_of(top) + value_of(warp_max_key(second)));
-        }
-      }
-      if (lane == g) mine = score;
-    }
-    unsigned keep = 0;
-    for (int r = 0; r < p.topk_groups; ++r) {
-      const Key top = warp_max_key(mine);
-      const int g = __ffs(__ballot_sync(FULL, mine == top)) - 1;
-      keep |= 1u << g;
-      if (lane == g) mine = 0;
-    }
-#pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (grp[i] < 0 || !(keep >> grp[i] & 1u)) key[i] = 0;
-  }
-  int mine_e = 0;
-  for (int j = 0; j < p.k; ++j) {
-    Key best = 0;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) best = key[i] > best ? key[i] : best;
-    const Key top = warp_max_key(best);
-    int at = p.E;
-#pragma unroll
-    for (int i = VPL - 1; i >= 0; --i)
-      if (key[i] == top) at = i * 32 + lane;
-    const int e = (int)__reduce_min_sync(FULL, (unsigned)at);
-#pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (e == i * 32 + lane) key[i] = 0;
-    if (lane == j) mine_e = e;
-  }
   float row_sum = 1.f;
-  if (!p.sigmoid && !p.renorm) {
+  if (!p.sigmoid && (SCORED || !p.renorm)) {
     row_sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) row_sum += z[i] == -INFINITY ? 0.f : __expf(z[i] - m);
     row_sum = warp_sum(row_sum);
   }
+  uint32_t key[VPL];
+  bool close = false;
+  int mine;
+  if constexpr (!SCORED) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) key[i] = i * 32 + lane < p.E ? key_of(z[i]) : 0u;
+    if (p.n_groups > 1) {
+      bool exact = false;  // a group counts its largest logit: nothing is rounded
+      only_groups(key, p, lane, best_groups(key, p, lane, exact));
+    }
+    mine = take_best<VPL, uint32_t, T, false>(key, p, zrow, lane, close);
+  } else {
+    const float inv = row_sum > 0.f ? 1.f / row_sum : 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      float c = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-z[i])) : __expf(z[i] - m) * inv;
+      c = z[i] == -INFINITY ? -INFINITY : c + b[i];
+      key[i] = i * 32 + lane < p.E ? key_of(c) : 0u;
+    }
+    if (p.n_groups > 1) {
+      const unsigned keep = best_groups(key, p, lane, close);
+      if (!p.bias) {  // inside the groups the logits tell the order
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+          if (key[i]) key[i] = key_of(z[i]);
+      }
+      only_groups(key, p, lane, keep);
+    }
+    mine = p.bias ? take_best<VPL, uint32_t, T, true>(key, p, zrow, lane, close) : take_best<VPL, uint32_t, T, false>(key, p, zrow, lane, close);
+    if (close) mine = rank_wide<VPL, T>(p, zrow, lane, m);  // uniform in the warp
+  }
   const bool slot = lane < p.k;
-  const float zs = slot ? to_f(zrow[mine_e]) : -INFINITY;
-  const bool dis = !slot || zs == -INFINITY || (p.bias && p.bias[mine_e] == -INFINITY);
+  const float zs = slot ? to_f(zrow[mine]) : -INFINITY;
+  const bool dis = !slot || zs == -INFINITY || (p.bias && p.bias[mine] == -INFINITY);
   float om;
   const float w = p.scale * slot_weight(zs, dis, p.sigmoid, p.renorm, m, row_sum, &om);
   if (slot) {
-    p.ids[(size_t)t * p.k + lane] = mine_e;
+    p.ids[(size_t)t * p.k + lane] = mine;
     store_f(p.w, (size_t)t * p.k + lane, p.w_f32, w);
   }
 }
 
-// dz of one token (one warp): a sum over the selected slots, and for the softmax without renormalisation a
-// dense row.  Scores are recomputed from the logits in fp32.
+// dz of one token (one warp): the row is written once with what every expert gets (0, or the common term of the
+// softmax without renormalisation), then the selected experts' values over it.  Scores are recomputed in fp32.
 template <int VPL, typename T>
 __global__ void __launch_bounds__(256) route_bwd_kernel(const RouteParams p, const void* dw, T* dz) {
   const int lane = threadIdx.x & 31;
   const int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (t >= p.T) return;
   const T* zrow = static_cast<const T*>(p.z) + (size_t)t * p.ldz;
+  T* orow = dz + (size_t)t * p.E;
   const bool slot = lane < p.k;
   const int e = slot ? (int)p.ids[(size_t)t * p.k + lane] : 0;
   const float zs = slot ? to_f(zrow[e]) : -INFINITY;
   const float g = slot ? load_f(dw, (size_t)t * p.k + lane, p.w_f32) : 0.f;
   const bool dis = !slot || zs == -INFINITY || (p.bias && p.bias[e] == -INFINITY);
-  const bool dense = !p.sigmoid && !p.renorm;
-  float out[VPL];
-  float m = -INFINITY, row_sum = 1.f;
-  if (dense) {
+  const float gd = dis ? 0.f : g;
+  float om;
+  if (!p.sigmoid && !p.renorm) {
+    float z[VPL];
+    float m = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      out[i] = i * 32 + lane < p.E ? to_f(zrow[i * 32 + lane]) : -INFINITY;
-      m = isnan(out[i]) ? NAN : fmaxf(m, out[i]);
+      z[i] = i * 32 + lane < p.E ? to_f(zrow[i * 32 + lane]) : -INFINITY;
+      m = fmaxf(m, z[i]);
     }
     m = warp_max(m);
-    row_sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      out[i] = out[i] == -INFINITY ? 0.f : __expf(out[i] - m);
-      row_sum += out[i];
+      z[i] = z[i] == -INFINITY ? 0.f : __expf(z[i] - m);
+      sum += z[i];
     }
-    row_sum = warp_sum(row_sum);
-  }
-  float om;
-  const float w = slot_weight(zs, dis, p.sigmoid, p.renorm, m, row_sum, &om);
-  const float gd = dis ? 0.f : g;
-  const float mean = p.renorm || dense ? warp_sum(gd * w) : 0.f;
-  float d;  // this slot's own term
-  if (dense) d = p.scale * gd;
-  else d = p.scale * w * (p.sigmoid ? om : 1.f) * (gd - mean);
-  if (dis) d = 0.f;
-  const float inv = dense && row_sum > 0.f ? 1.f / row_sum : (row_sum == 0.f ? 0.f : row_sum);
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) out[i] = dense ? out[i] * inv : 0.f;
-  float own[VPL];
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) own[i] = 0.f;
-  for (int j = 0; j < p.k; ++j) {
-    const int ej = __shfl_sync(FULL, e, j);
-    const float dj = __shfl_sync(FULL, d, j);
+    sum = warp_sum(sum);
+    const float w = slot_weight(zs, dis, false, false, m, sum, &om);
+    const float mean = warp_sum(gd * w);
+    const float f = sum == 0.f ? 0.f : -p.scale * mean / sum;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-      if (ej == i * 32 + lane) own[i] = dj;
-  }
+      if (i * 32 + lane < p.E) from_f(orow + i * 32 + lane, z[i] * f);
+    __syncwarp();
+    if (!dis) from_f(orow + e, p.scale * w * (gd - mean));
+  } else {
+    const float w = slot_weight(zs, dis, p.sigmoid, p.renorm, 0.f, 1.f, &om);
+    const float mean = p.renorm ? warp_sum(gd * w) : 0.f;
+    const float d = dis ? 0.f : p.scale * w * om * (gd - mean);
+    constexpr int PER = 16 / sizeof(T);
+    if (p.E % PER == 0) {
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    const int c = i * 32 + lane;
-    if (c < p.E) from_f(dz + (size_t)t * p.E + c, dense ? out[i] * (own[i] - p.scale * mean) : own[i]);
+      for (int i = 0; i < (VPL * 32 + 32 * PER - 1) / (32 * PER); ++i)
+        if ((i * 32 + lane) * PER < p.E) reinterpret_cast<uint4*>(orow)[i * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (i * 32 + lane < p.E) from_f(orow + i * 32 + lane, 0.f);
+    }
+    __syncwarp();
+    if (slot) from_f(orow + e, d);
   }
 }
 
@@ -312,6 +382,7 @@ __device__ __forceinline__ int expert_of(const PlanParams& p, int a) {
 // Counts of each block's chunk; the rows are preset to "no assignment".
 __global__ void __launch_bounds__(PLAN_THREADS) plan_count_kernel(const PlanParams p) {
   __shared__ int h[1024];
+  await_predecessor();
   for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS) h[e] = 0;
   __syncthreads();
 #pragma unroll
@@ -349,6 +420,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
   __shared__ int red[32][2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint16_t* mine = wc + warp * p.E;
+  await_predecessor();
   for (int e = lane; e < p.E; e += 32) mine[e] = 0;
   if (SINGLE)
     for (int r = tid; r < p.R; r += PLAN_THREADS) p.rows[r] = -1;
@@ -376,15 +448,25 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
       in_block += c;
     }
   }
-  int total = in_block, before = 0;
-  if (!SINGLE && tid < p.E) {
-    total = 0;
-#pragma unroll 8
-    for (int b = 0; b < p.nb; ++b) {
-      const int c = p.hist[(size_t)b * p.E + tid];
-      if (b < (int)blockIdx.x) before += c;
-      total += c;
+  int total = SINGLE ? in_block : 0, before = 0;
+  if (!SINGLE) {  // totals over the blocks: the threads share the blocks of an expert
+    __shared__ int sum[1024], upto[1024];
+    sum[tid] = upto[tid] = 0;
+    __syncthreads();
+    const int parts = PLAN_THREADS / p.E, part = tid / p.E, e = tid - part * p.E;
+    if (part < parts) {
+#pragma unroll 16
+      for (int b = part; b < p.nb; b += parts) {
+        const int c = p.hist[(size_t)b * p.E + e];
+        before += b < (int)blockIdx.x ? c : 0;
+        total += c;
+      }
+      atomicAdd(&sum[e], total);
+      atomicAdd(&upto[e], before);
     }
+    __syncthreads();
+    total = sum[tid];
+    before = upto[tid];
   }
   if (tid >= p.E) total = 0;
   const int padded = (total + ALIGN - 1) / ALIGN * ALIGN;
@@ -423,6 +505,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
 __global__ void __launch_bounds__(256) gather_kernel(const __nv_bfloat16* src, long ld, const int* rows, const int* end, const void* w, int w_f32,
                                                      float* rw, __nv_bfloat16* dst, int k, int D) {
   const int lane = threadIdx.x & 31;
+  await_predecessor();
   const int last = *end;
   for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < last; r += gridDim.x * 8) {
     const int a = rows[r];
@@ -442,6 +525,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const __nv_bfloat16* src, l
 // With `part`: dweights[t][j] = sum over the feature tiles of its row's partial dot products.
 __global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, const int* slots, const __nv_bfloat16* res, long ldr, __nv_bfloat16* out,
                                                       const float* part, int n_part, void* dw, int w_f32, int T, int k, int D) {
+  await_predecessor();
   const int per = D / 8;
   const int lanes = per < 256 ? per : 256;  // threads that share a token
   const int groups = 256 / lanes;
@@ -502,16 +586,16 @@ int route_check(const RouteParams& p) {
   return KB_STATUS_OK;
 }
 
-template <typename T, typename Key>
+template <typename T, bool SCORED>
 void route_fwd(const RouteParams& p, cudaStream_t st) {
   const int grid = (p.T + 7) / 8;
   const int vpl = (p.E + 31) / 32;
-  if (vpl <= 1) route_fwd_kernel<1, T, Key><<<grid, 256, 0, st>>>(p);
-  else if (vpl <= 2) route_fwd_kernel<2, T, Key><<<grid, 256, 0, st>>>(p);
-  else if (vpl <= 4) route_fwd_kernel<4, T, Key><<<grid, 256, 0, st>>>(p);
-  else if (vpl <= 8) route_fwd_kernel<8, T, Key><<<grid, 256, 0, st>>>(p);
-  else if (vpl <= 16) route_fwd_kernel<16, T, Key><<<grid, 256, 0, st>>>(p);
-  else route_fwd_kernel<32, T, Key><<<grid, 256, 0, st>>>(p);
+  if (vpl <= 1) route_fwd_kernel<1, T, SCORED><<<grid, 256, 0, st>>>(p);
+  else if (vpl <= 2) route_fwd_kernel<2, T, SCORED><<<grid, 256, 0, st>>>(p);
+  else if (vpl <= 4) route_fwd_kernel<4, T, SCORED><<<grid, 256, 0, st>>>(p);
+  else if (vpl <= 8) route_fwd_kernel<8, T, SCORED><<<grid, 256, 0, st>>>(p);
+  else if (vpl <= 16) route_fwd_kernel<16, T, SCORED><<<grid, 256, 0, st>>>(p);
+  else route_fwd_kernel<32, T, SCORED><<<grid, 256, 0, st>>>(p);
 }
 template <typename T>
 void route_bwd(const RouteParams& p, const void* dw, void* dz, cudaStream_t st) {
@@ -533,11 +617,9 @@ extern "C" int kb_moe_route_fwd(const void* z, int z_f32, long ldz, const float*
   if (const int rc = route_check(p)) return rc;
   if (T == 0) return KB_STATUS_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Without a bias and without sums of group scores the order of the scores is the order of the logits; else
-  // scores next to the border of the k largest need more than fp32 to be told apart.
-  const bool wide = bias != nullptr || (n_groups > 1 && group_top == 2 && E / n_groups > 1);
-  if (z_f32) wide ? route_fwd<float, uint64_t>(p, st) : route_fwd<float, uint32_t>(p, st);
-  else wide ? route_fwd<__nv_bfloat16, uint64_t>(p, st) : route_fwd<__nv_bfloat16, uint32_t>(p, st);
+  const bool scored = bias != nullptr || (n_groups > 1 && group_top == 2 && E / n_groups > 1);
+  if (z_f32) scored ? route_fwd<float, true>(p, st) : route_fwd<float, false>(p, st);
+  else scored ? route_fwd<__nv_bfloat16, true>(p, st) : route_fwd<__nv_bfloat16, false>(p, st);
   return launched();
 }
 
@@ -563,15 +645,15 @@ extern "C" int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int*
   PlanParams p{ids, ids64, n, E, R, nb, counts, offsets, slots, rows, reinterpret_cast<int4*>(tiles), hist};
   const int smem = 32 * E * 2;
   if (nb == 1) {
-    if (smem > 40 * 1024 && cudaFuncSetAttribute(plan_place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    if (smem > 32 * 1024 && cudaFuncSetAttribute(plan_place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return KB_STATUS_CUDA_ERROR;
-    plan_place_kernel<true><<<1, PLAN_THREADS, smem, st>>>(p);
+    launch_after(plan_place_kernel<true>, 1, PLAN_THREADS, smem, st, p);
   } else {
     if (hist == nullptr) return KB_STATUS_BAD_ARG;
-    if (smem > 40 * 1024 && cudaFuncSetAttribute(plan_place_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    if (smem > 32 * 1024 && cudaFuncSetAttribute(plan_place_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return KB_STATUS_CUDA_ERROR;
-    plan_count_kernel<<<nb, PLAN_THREADS, 0, st>>>(p);
-    plan_place_kernel<false><<<nb, PLAN_THREADS, smem, st>>>(p);
+    launch_after(plan_count_kernel, nb, PLAN_THREADS, 0, st, p);
+    launch_after(plan_place_kernel<false>, nb, PLAN_THREADS, smem, st, p);
   }
   return launched();
 }
@@ -583,16 +665,16 @@ namespace moe {
 int launch_gather(const void* src, long ld, const int* rows, const int* end, const void* w, int w_f32, float* rw, void* dst, int k, int D, int R, int sms,
                   cudaStream_t st) {
   const int want = (R + 7) / 8, cap = sms * 8;
-  gather_kernel<<<want < cap ? want : cap, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(src), ld, rows, end, w, w_f32, rw,
-                                                         static_cast<__nv_bfloat16*>(dst), k, D);
+  launch_after(gather_kernel, want < cap ? want : cap, 256, 0, st, static_cast<const __nv_bfloat16*>(src), ld, rows, end, w, w_f32, rw,
+               static_cast<__nv_bfloat16*>(dst), k, D);
   return launched();
 }
 
 int launch_combine(const void* y, const int* slots, const void* res, long ldr, void* out, const float* part, int n_part, void* dw, int w_f32, int T, int k,
                    int D, cudaStream_t st) {
   const int per = D / 8, lanes = per < 256 ? per : 256, groups = 256 / lanes;
-  combine_kernel<<<(T + groups - 1) / groups, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(y), slots, static_cast<const __nv_bfloat16*>(res), ldr,
-                                                            static_cast<__nv_bfloat16*>(out), part, n_part, dw, w_f32, T, k, D);
+  launch_after(combine_kernel, (T + groups - 1) / groups, 256, 0, st, static_cast<const __nv_bfloat16*>(y), slots,
+               static_cast<const __nv_bfloat16*>(res), ldr, static_cast<__nv_bfloat16*>(out), part, n_part, dw, w_f32, T, k, D);
   return launched();
 }
 

@@ -5,6 +5,29 @@
 namespace kb {
 namespace moe {
 
+// The kernels of a pass follow one another with programmatic launch: a kernel may start while its predecessor
+// still drains and waits here for the predecessor's results, before it touches memory that others write.  The
+// successor is let in behind that wait, so a kernel that runs knows that everything before its direct
+// predecessor has completed.
+__device__ __forceinline__ void await_predecessor() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... KArgs, typename... Args>
+cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args&&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
 // dst[r] = src[rows[r] / k] for the first *end rows (zero where rows[r] < 0); rw[r]: the row's routing weight.
 int launch_gather(const void* src, long ld, const int* rows, const int* end, const void* w, int w_f32, float* rw, void* dst, int k, int D, int R, int sms,
                   cudaStream_t st);

@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import check, lib, stream
+from ._lib import check, lib
 from .functional import _count_use, _use_done
 
 ROW_ALIGN = 16      # an expert's segment of the grouped rows begins on a multiple of this
@@ -26,16 +26,18 @@ TILE_ROWS = 128     # rows of one tile of the grouped products
 MAX_EXPERTS = 1024
 MAX_SLOTS = 32      # experts per token, and groups of experts
 PLAN_CHUNK = 4096   # assignments that one block of the grouping kernel takes
+SMALL = 32          # assignments up to which a forward pass without gradients needs no grouping
 
 Stack = Union[Tensor, Sequence[Tensor]]
 
 
 def _call(t: Tensor, name: str, *args) -> None:
     """One entry of the kernel library on the current stream of ``t``'s device."""
-    if t.get_device() != torch.cuda.current_device():
-        with torch.cuda.device(t.device):
+    dev = t.get_device()
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
             return _call(t, name, *args)
-    check(getattr(lib(), name)(*args, stream()), name[3:])
+    check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(dev)), name[3:])
 
 
 def _p(t: Optional[Tensor]):
@@ -347,7 +349,7 @@ class _ExpertsFn(torch.autograd.Function):
         dout = _rows2d(dout)
         dev = dout.device
         need = ctx.needs_input_grad
-        n_part = -(-F // 256)
+        n_part = 2 * -(-F // 256)
         sp = _Space(dev, dys=2 * R * D, dg=2 * R * F, du=2 * R * F, part=4 * R * n_part)
         dx = torch.empty((T, D), dtype=dout.dtype, device=dev) if need[0] else None
         dw = torch.empty((T, k), dtype=w_dtype, device=dev) if need[1] else None
@@ -378,6 +380,17 @@ class _ExpertsFn(torch.autograd.Function):
                     wanted = need[6 + i * n_each + j]
                     out.append((grads[i] if group[0].dim() == 3 else grads[i][j]) if wanted else None)
         return (dx, dw, dout if need[2] else None, None, None, None, *out)
+
+
+def _experts_small(x, w, ids, res, wg, wu, wd) -> Tensor:
+    (T, D), k, (E, F, _) = x.shape, w.shape[1], wg.shape
+    out = torch.empty((T, D), dtype=x.dtype, device=x.device)
+    h = torch.empty((T * k, F), dtype=torch.float32, device=x.device)
+    _call(x, "kb_moe_experts_small", _p(x), x.stride(0), _p(w), int(w.dtype == torch.float32), _p(ids), int(ids.dtype == torch.int64), _p(wg), wg.stride(1),
+          _stride0(wg), _p(wu), wu.stride(1), _stride0(wu), _p(wd), wd.stride(1), _stride0(wd), _p(res), res.stride(0) if res is not None else 0, _p(out), _p(h),
+          T, k, D, F, E)
+    _lib.add_launches(1)
+    return out
 
 
 def _rows2d(t: Tensor) -> Tensor:
@@ -438,6 +451,8 @@ def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up
               and weights.dtype in (torch.bfloat16, torch.float32) and (r2 is None or r2.dtype == torch.bfloat16) and ids2.numel() > 0)
     if not kernel:
         return _experts_torch(x2, w2, ids2, *(s[0] if lone else s for s in stacks), r2).view(x.shape)
-    plan = moe_plan(ids2, E) if plan is None else plan
     train = torch.is_grad_enabled() and any(t.requires_grad for t in (x2, w2, *every, *([r2] if r2 is not None else [])))
+    if not train and ids2.numel() <= SMALL:
+        return _experts_small(_rows2d(x2), w2.contiguous(), ids2.contiguous(), None if r2 is None else _rows2d(r2), *(_stacked(s) for s in stacks)).view(x.shape)
+    plan = moe_plan(ids2, E) if plan is None else plan
     return _ExpertsFn.apply(_rows2d(x2), w2.contiguous(), None if r2 is None else _rows2d(r2), plan, n_each, train, *every).view(x.shape)
