@@ -204,7 +204,7 @@ int kb_gemm_comm(const void* const* a_ptrs, const void* const* b_ptrs, void* c_l
 #define KB_MOE_ROW_ALIGN 16      // an expert's segment of the grouped rows begins on a multiple of this
 #define KB_MOE_TILE_ROWS 128     // rows of a tile of the grouped products
 #define KB_MOE_MAX_EXPERTS 1024
-#define KB_MOE_SMALL_MAX 32      // assignments that the small form takes
+#define KB_MOE_SMALL_MAX 16      // assignments that the small form takes
 // Routing: weights [T,k] and experts [T,k] (int64) of logits [T,E] (bf16 or fp32, pitch ldz); bias [E] or NULL is added
 // for the selection only.  k <= 32, n_groups <= 32, group_top 1 or 2.
 int kb_moe_route_fwd(const void* z, int z_f32, long ldz, const float* bias, void* w, int w_f32, long long* ids, int T, int E, int k,
@@ -213,7 +213,7 @@ int kb_moe_route_fwd(const void* z, int z_f32, long ldz, const float* bias, void
 int kb_moe_route_bwd(const void* z, int z_f32, long ldz, const float* bias, const long long* ids, const void* dw, int w_f32, void* dz,
                      int T, int E, int k, int sigmoid, int renorm, float scale, void* stream);
 // Grouping of n assignments by expert.  counts [E], offsets [E+1], slots [n], rows [R], tiles [1 + tiles][4] (16-byte aligned,
-// R / 128 + min(E, n) tiles at most); R >= n + 15 min(E, n) rounded up to 16; hist [ceil(n / 4096), E] scratch (n > 4096).
+// R / 128 + min(E, n) tiles at most); R >= n + 15 min(E, n) rounded up to 16; hist [ceil(n / 2048), E] scratch (n > 2048).
 // An index outside 0..E-1 is dropped (slot -1).
 int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int* counts, int* offsets, int* slots, int* rows, int* tiles, int* hist,
                 void* stream);

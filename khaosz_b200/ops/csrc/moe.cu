@@ -355,11 +355,11 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const RouteParams p, con
 // ---------------------------------------------------------------------------------------
 // grouping
 // ---------------------------------------------------------------------------------------
-// Stable counting sort without atomics on the result: a block owns CHUNK consecutive assignments, a warp 128
-// of them in four steps of 32; __match_any_sync ranks equal experts inside a step, per-warp counters in shared
+// Stable counting sort without atomics on the result: a block owns CHUNK consecutive assignments, a warp 64
+// of them in two steps of 32; __match_any_sync ranks equal experts inside a step, per-warp counters in shared
 // memory carry the rank over the steps, a prefix over the warps and over the blocks completes it.
 constexpr int PLAN_THREADS = 1024;
-constexpr int STEPS = 4;
+constexpr int STEPS = 2;
 constexpr int CHUNK = PLAN_THREADS * STEPS;
 
 struct PlanParams {

@@ -13,8 +13,8 @@ namespace moe_small {
 
 constexpr unsigned FULL = 0xffffffffu;
 constexpr int WARPS = 8;
-constexpr int MEMBERS = 4;  // tokens of an expert that share one pass over its weight rows
 constexpr int PIECES = 4;   // 16-byte pieces of each row that a lane has in flight
+constexpr int ROWS = 2;     // rows of the down projection that a warp takes, so that h is read half as often
 
 struct Params {
   const __nv_bfloat16 *x, *wg, *wu, *wd, *res;
@@ -45,7 +45,9 @@ __device__ __forceinline__ uint4 stream_load(const uint4* p) {  // weights are r
   return v;
 }
 
-// h[a][f] = w[a] * silu(x[t] . gate[e][f]) * (x[t] . up[e][f]); the first assignment of an expert does them all.
+// h[a][f] = w[a] * silu(x[t] . gate[e][f]) * (x[t] . up[e][f]); the first assignment of an expert does them all,
+// MEMBERS tokens in one pass over its rows (1 for a single token: half the registers, twice the warps in flight).
+template <int MEMBERS>
 __global__ void __launch_bounds__(WARPS * 32) up_kernel(const Params p) {
   const int lane = threadIdx.x & 31, n = p.T * p.k;
   kb::moe::await_predecessor();
@@ -106,52 +108,63 @@ __global__ void __launch_bounds__(WARPS * 32) up_kernel(const Params p) {
   }
 }
 
-// out[t][d] = res[t][d] + sum_j h[t][j] . down[e_j][d]; `split` warps of the block share one d.
+// out[t][d] = res[t][d] + sum_j h[t][j] . down[e_j][d]; `split` warps of the block share ROWS features.
 __global__ void __launch_bounds__(WARPS * 32) down_kernel(const Params p, int split) {
-  __shared__ float part[WARPS];
+  __shared__ float part[WARPS][ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int d = blockIdx.x * (WARPS / split) + warp / split;
+  const int d0 = (blockIdx.x * (WARPS / split) + warp / split) * ROWS;
   const int t = blockIdx.y;
-  float s = 0.f;
+  float s[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) s[r] = 0.f;
   bool waited = false;
-  if (d < p.D) {
+  if (d0 < p.D) {  // D is a multiple of 8
     const int pieces = p.F / 8;
     for (int j = warp % split; j < p.k; j += split) {
       const int a = t * p.k + j;
       const int e = expert_of(p, a);
       if (e < 0) continue;
-      const uint4* wrow = reinterpret_cast<const uint4*>(p.wd + e * p.sd + d * p.ldd);
+      const __nv_bfloat16* w0 = p.wd + e * p.sd + d0 * p.ldd;
       const float4* hrow = reinterpret_cast<const float4*>(p.h + (size_t)a * p.F);
-      for (int c0 = lane; c0 < pieces; c0 += 32 * 2 * PIECES) {
-        uint4 v[2 * PIECES];
+      for (int c0 = lane; c0 < pieces; c0 += 32 * PIECES) {
+        uint4 v[ROWS][PIECES];
 #pragma unroll
-        for (int q = 0; q < 2 * PIECES; ++q) v[q] = c0 + q * 32 < pieces ? stream_load(wrow + c0 + q * 32) : make_uint4(0u, 0u, 0u, 0u);
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+          for (int q = 0; q < PIECES; ++q)
+            v[r][q] = c0 + q * 32 < pieces ? stream_load(reinterpret_cast<const uint4*>(w0 + r * p.ldd) + c0 + q * 32) : make_uint4(0u, 0u, 0u, 0u);
         if (!waited) {  // the first weights are under way while the hidden activations are still computed
           kb::moe::await_predecessor();
           waited = true;
         }
 #pragma unroll
-        for (int q = 0; q < 2 * PIECES; ++q) {
+        for (int q = 0; q < PIECES; ++q) {
           const int c = c0 + q * 32;
           if (c >= pieces) break;
           const float4 a0 = hrow[2 * c], a1 = hrow[2 * c + 1];
-          const float2 w0 = unpack_bf16x2(v[q].x), w1 = unpack_bf16x2(v[q].y), w2 = unpack_bf16x2(v[q].z), w3 = unpack_bf16x2(v[q].w);
-          s = fmaf(a0.x, w0.x, s); s = fmaf(a0.y, w0.y, s); s = fmaf(a0.z, w1.x, s); s = fmaf(a0.w, w1.y, s);
-          s = fmaf(a1.x, w2.x, s); s = fmaf(a1.y, w2.y, s); s = fmaf(a1.z, w3.x, s); s = fmaf(a1.w, w3.y, s);
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            const float2 x0 = unpack_bf16x2(v[r][q].x), x1 = unpack_bf16x2(v[r][q].y), x2 = unpack_bf16x2(v[r][q].z), x3 = unpack_bf16x2(v[r][q].w);
+            s[r] = fmaf(a0.x, x0.x, s[r]); s[r] = fmaf(a0.y, x0.y, s[r]); s[r] = fmaf(a0.z, x1.x, s[r]); s[r] = fmaf(a0.w, x1.y, s[r]);
+            s[r] = fmaf(a1.x, x2.x, s[r]); s[r] = fmaf(a1.y, x2.y, s[r]); s[r] = fmaf(a1.z, x3.x, s[r]); s[r] = fmaf(a1.w, x3.y, s[r]);
+          }
         }
       }
     }
-    s = warp_sum(s);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) s[r] = warp_sum(s[r]);
   }
   if (!waited) kb::moe::await_predecessor();
-  if (lane == 0) part[warp] = s;
+  if (lane < ROWS) part[warp][lane] = lane ? s[ROWS - 1] : s[0];
   __syncthreads();
-  if (lane == 0 && d < p.D && warp % split == 0) {
+  if (lane < ROWS && d0 < p.D && warp % split == 0) {
+    const int d = d0 + lane;
     float total = p.res ? __bfloat162float(p.res[t * p.ldr + d]) : 0.f;
-    for (int i = 0; i < split; ++i) total += part[warp + i];
+    for (int i = 0; i < split; ++i) total += part[warp + i][lane];
     p.out[(size_t)t * p.D + d] = __float2bfloat16(total);
   }
 }
+static_assert(ROWS == 2, "part[] is filled by two lanes");
 
 }  // namespace moe_small
 }  // namespace kb
@@ -169,8 +182,8 @@ extern "C" int kb_moe_experts_small(const void* x, long ldx, const void* weights
   const Params p{static_cast<bf>(x), static_cast<bf>(wg), static_cast<bf>(wu), static_cast<bf>(wd), static_cast<bf>(res), weights, ids,
                  static_cast<__nv_bfloat16*>(out), h, ldx, ldg, sg, ldu, su, ldd, sd, ldr, w_f32, ids64, T, k, D, F, E};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  kb::moe::launch_after(up_kernel, dim3((F + WARPS - 1) / WARPS, T * k), WARPS * 32, 0, st, p);
+  kb::moe::launch_after(T == 1 ? up_kernel<1> : up_kernel<4>, dim3((F + WARPS - 1) / WARPS, T * k), WARPS * 32, 0, st, p);
   const int split = k >= 8 ? 8 : k >= 4 ? 4 : k >= 2 ? 2 : 1;
-  kb::moe::launch_after(down_kernel, dim3((D + WARPS / split - 1) / (WARPS / split), T), WARPS * 32, 0, st, p, split);
+  kb::moe::launch_after(down_kernel, dim3((D / ROWS + WARPS / split - 1) / (WARPS / split), T), WARPS * 32, 0, st, p, split);
   return cudaGetLastError() == cudaSuccess ? KB_STATUS_OK : KB_STATUS_CUDA_ERROR;
 }

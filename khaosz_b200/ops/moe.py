@@ -25,9 +25,10 @@ ROW_ALIGN = 16      # an expert's segment of the grouped rows begins on a multip
 TILE_ROWS = 128     # rows of one tile of the grouped products
 MAX_EXPERTS = 1024
 MAX_SLOTS = 32      # experts per token, and groups of experts
-PLAN_CHUNK = 4096   # assignments that one block of the grouping kernel takes
-SMALL = 32          # assignments up to which a forward pass without gradients needs no grouping
+PLAN_CHUNK = 2048   # assignments that one block of the grouping kernel takes
+SMALL = 16          # assignments up to which a forward pass without gradients needs no grouping (see _experts_small)
 
+_KERNEL_DTYPES = (torch.bfloat16, torch.float32)
 Stack = Union[Tensor, Sequence[Tensor]]
 
 
@@ -105,28 +106,33 @@ def _route_torch(z, bias, k, sigmoid, n_groups, topk_groups, group_top, renormal
     return w.to(dtype), ids
 
 
+def _route_kernel(z, bias, k, sigmoid, n_groups, topk_groups, group_top, renormalize, scale, dtype):
+    T, E = z.shape
+    w = torch.empty((T, k), dtype=dtype, device=z.device)
+    ids = torch.empty((T, k), dtype=torch.long, device=z.device)
+    _call(z, "kb_moe_route_fwd", z.data_ptr(), z.dtype == torch.float32, z.stride(0), _p(bias), w.data_ptr(), dtype == torch.float32, ids.data_ptr(), T, E, k,
+          sigmoid, renormalize, n_groups, topk_groups, group_top, scale)
+    return w, ids
+
+
 class _RouteFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, bias, k, sigmoid, n_groups, topk_groups, group_top, renormalize, scale, dtype):
-        T, E = z.shape
-        w = torch.empty((T, k), dtype=dtype, device=z.device)
-        ids = torch.empty((T, k), dtype=torch.long, device=z.device)
-        f32, w32 = int(z.dtype == torch.float32), int(dtype == torch.float32)
-        _call(z, "kb_moe_route_fwd", _p(z), f32, z.stride(0), _p(bias), _p(w), w32, _p(ids), T, E, k, int(sigmoid), int(renormalize), n_groups,
-              topk_groups, group_top, scale)
+    def forward(ctx, z, bias, *args):
+        w, ids = _route_kernel(z, bias, *args)
         ctx.save_for_backward(z, bias, ids)
-        ctx.args = (k, int(sigmoid), int(renormalize), scale, f32, w32)
+        ctx.args = args
         ctx.mark_non_differentiable(ids)
         return w, ids
 
     @staticmethod
     def backward(ctx, dw, _):
         z, bias, ids = ctx.saved_tensors
-        k, sigmoid, renormalize, scale, f32, w32 = ctx.args
+        k, sigmoid, _, _, _, renormalize, scale, dtype = ctx.args
         T, E = z.shape
         dw = dw.contiguous()
         dz = torch.empty((T, E), dtype=z.dtype, device=z.device)
-        _call(z, "kb_moe_route_bwd", _p(z), f32, z.stride(0), _p(bias), _p(ids), _p(dw), w32, _p(dz), T, E, k, sigmoid, renormalize, scale)
+        _call(z, "kb_moe_route_bwd", z.data_ptr(), z.dtype == torch.float32, z.stride(0), _p(bias), ids.data_ptr(), dw.data_ptr(), dtype == torch.float32,
+              dz.data_ptr(), T, E, k, sigmoid, renormalize, scale)
         return (dz,) + (None,) * 9
 
 
@@ -158,16 +164,19 @@ def moe_route(logits: Tensor, k: int, *, score: str = "softmax", bias: Optional[
     if bias is not None and (bias.shape != (E,) or not bias.is_floating_point() or bias.device != logits.device):
         raise ValueError("moe_route: bias must be a floating-point tensor [experts] on the logits' device")
     dtype = logits.dtype if dtype is None else dtype
-    lead = logits.shape[:-1]
-    z = logits.reshape(-1, E)
+    z = logits if logits.dim() == 2 else logits.reshape(-1, E)
     args = (int(k), score == "sigmoid", int(n_groups), int(topk_groups), int(group_top), bool(renormalize), float(scale), dtype)
-    if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32) or dtype not in (torch.bfloat16, torch.float32):
+    if not logits.is_cuda or logits.dtype not in _KERNEL_DTYPES or dtype not in _KERNEL_DTYPES:
         w, ids = _route_torch(z, bias, *args)
     else:
-        if z.stride(-1) != 1 and E > 1 or z.stride(0) < E:
+        if z.stride(1) != 1 and E > 1 or z.stride(0) < E:
             z = z.contiguous()
-        w, ids = _RouteFn.apply(z, None if bias is None else bias.detach().float().contiguous(), *args)
-    return w.view(*lead, k), ids.view(*lead, k)
+        if bias is not None:
+            bias = bias.detach()
+            if bias.dtype != torch.float32 or not bias.is_contiguous():
+                bias = bias.float().contiguous()
+        w, ids = _RouteFn.apply(z, bias, *args) if z.requires_grad and torch.is_grad_enabled() else _route_kernel(z, bias, *args)
+    return (w, ids) if logits.dim() == 2 else (w.view(*logits.shape[:-1], k), ids.view(*logits.shape[:-1], k))
 
 
 # ---------------------------------------------------------------------------------------
@@ -241,12 +250,16 @@ def moe_plan(experts: Tensor, n_experts: int) -> MoEPlan:
     ids = experts.contiguous()
     R, blocks = rows_bound(n, E), -(-n // PLAN_CHUNK)
     # tiles come first: they are read as 16-byte entries
-    sizes = [4 * (1 + _tiles_bound(n, E)), E, E + 1, n, R] + ([blocks * E] if blocks > 1 else [])
-    parts = torch.empty(sum(sizes), dtype=torch.int32, device=ids.device).split(sizes)
-    tiles, counts, offsets, slots, rows = parts[:5]
-    _call(ids, "kb_moe_plan", _p(ids), int(ids.dtype == torch.int64), n, E, R, _p(counts), _p(offsets), _p(slots), _p(rows), _p(tiles),
-          _p(parts[5]) if blocks > 1 else None)
+    sizes = [4 * (1 + _tiles_bound(n, E)), E, E + 1, n, R]
     if blocks > 1:
+        sizes.append(blocks * E)
+    tiles, counts, offsets, slots, rows, *hist = torch.empty(sum(sizes), dtype=torch.int32, device=ids.device).split_with_sizes(sizes)
+    at = tiles.data_ptr()
+    o = [at]
+    for z in sizes:
+        o.append(o[-1] + 4 * z)
+    _call(ids, "kb_moe_plan", ids.data_ptr(), ids.dtype == torch.int64, n, E, R, o[1], o[2], o[3], o[4], at, o[5] if hist else None)
+    if hist:
         _lib.add_launches(1)
     return MoEPlan(counts, offsets, slots.view(experts.shape), rows, tiles.view(-1, 4))
 
@@ -257,31 +270,37 @@ def moe_plan(experts: Tensor, n_experts: int) -> MoEPlan:
 
 
 def _uniform(ws: Sequence[Tensor]) -> Optional[Tensor]:
-    """The ``[E, rows, cols]`` view over equally spaced matrices of one storage, if they are that."""
-    first = ws[0]
-    base, size = first.untyped_storage().data_ptr(), first.element_size()
-    at = first.data_ptr()
-    step = ws[1].data_ptr() - at if len(ws) > 1 else first.numel() * size
-    if step < first.numel() * size or step % size:
+    """The ``[E, rows, cols]`` view over equally spaced contiguous matrices of one storage, if they are that."""
+    first = ws[0].detach()
+    shape, size, n = first.shape, first.element_size(), len(ws)
+    at = [w.data_ptr() for w in ws]
+    step = at[1] - at[0] if n > 1 else first.numel() * size
+    if step < first.numel() * size or step % size or at != list(range(at[0], at[0] + n * step, step)):
         return None
-    for w in ws:
-        if w.data_ptr() != at or w.shape != first.shape or w.dtype != first.dtype or not w.is_contiguous() or w.untyped_storage().data_ptr() != base:
-            return None
-        at += step
-    return first.detach().as_strided((len(ws), *first.shape), (step // size, first.shape[1], 1), first.storage_offset())
+    if any(w.shape != shape or w.dtype != first.dtype or not w.is_contiguous() for w in ws):
+        return None
+    # separate allocations can touch by accident: all of it has to lie in the first one's storage
+    if first.storage_offset() * size + (n - 1) * step + first.numel() * size > first.untyped_storage().nbytes():
+        return None
+    return first.as_strided((n, *shape), (step // size, shape[1], 1), first.storage_offset())
 
 
 def _kernel_view(w: Tensor) -> Tensor:
     """``w [E, rows, cols]`` as the kernels read it: unit inner stride, pitch and distance in multiples of 16 bytes."""
     E, _, cols = w.shape
-    if (w.stride(2) != 1 or w.stride(1) < cols or w.stride(1) % 8 or w.data_ptr() % 16
-            or (E > 1 and (w.stride(0) < cols or w.stride(0) % 8))):
+    s0, s1, s2 = w.stride()
+    if s2 != 1 or s1 < cols or s1 % 8 or w.data_ptr() % 16 or (E > 1 and (s0 < cols or s0 % 8)):
         return w.contiguous()
     return w
 
 
 def _stride0(w: Tensor) -> int:
     return w.stride(0) if w.shape[0] > 1 else w.shape[1] * w.stride(1)
+
+
+def _where(w: Tensor) -> Tuple[int, int, int]:
+    """Address, pitch and distance of the experts."""
+    return w.data_ptr(), w.stride(1), _stride0(w)
 
 
 def _stacked(group: Sequence[Tensor]) -> Tensor:
@@ -309,65 +328,66 @@ class _Space:
         for name, nbytes in sizes.items():
             self.offset[name] = at
             at += _round_up(nbytes, 256)
-        self.buf = torch.empty(max(at, 1), dtype=torch.uint8, device=device)
+        self.buf = torch.empty(at, dtype=torch.uint8, device=device)
 
     def __getitem__(self, name: str):
         return self.buf.data_ptr() + self.offset[name] if name in self.offset else None
 
 
+def _experts_forward(x, weights, residual, plan, groups, train):
+    """(out, scratch, stacked weights); with ``train`` the scratch keeps what the backward pass reads."""
+    wg, wu, wd = (_stacked(g) for g in groups)
+    (T, D), k, E, F, R = x.shape, weights.shape[1], wg.shape[0], wg.shape[1], plan.rows.numel()
+    wide, hidden = 2 * R * D, 2 * R * F
+    if train:
+        sp = _Space(x.device, xs=wide, rw=4 * R, h=hidden, g=hidden, u=hidden)
+        ys = torch.empty(wide, dtype=torch.uint8, device=x.device)
+        y = ys.data_ptr()
+    else:   # nobody reads the grouped inputs again: the experts' outputs overwrite them
+        sp = _Space(x.device, xs=wide, rw=4 * R, h=hidden)
+        y = sp["xs"]
+    out = torch.empty((T, D), dtype=x.dtype, device=x.device)
+    _call(x, "kb_moe_experts_fwd", x.data_ptr(), x.stride(0), weights.data_ptr(), weights.dtype == torch.float32, plan.offsets.data_ptr(),
+          plan.slots.data_ptr(), plan.rows.data_ptr(), plan.tiles.data_ptr(), *_where(wg), *_where(wu), *_where(wd), _p(residual),
+          0 if residual is None else residual.stride(0), out.data_ptr(), sp["xs"], sp["rw"], sp["g"], sp["u"], sp["h"], y, T, k, D, F, E, R)
+    _lib.add_launches(3)
+    return out, sp, (wg, wu, wd)
+
+
 class _ExpertsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weights, residual, plan, n_each, train, *ws):
+    def forward(ctx, x, weights, residual, plan, n_each, *ws):
         groups = [ws[i * n_each:(i + 1) * n_each] for i in range(3)]
-        wg, wu, wd = (_stacked(g) for g in groups)
-        (T, D), k, E, F = x.shape, weights.shape[1], wg.shape[0], wg.shape[1]
-        R = plan.rows.numel()
-        wide, hidden = 2 * R * D, 2 * R * F
-        sp = _Space(x.device, xs=wide, rw=4 * R, h=hidden, **(dict(g=hidden, u=hidden) if train else {}))
-        out = torch.empty((T, D), dtype=x.dtype, device=x.device)
-        # without a backward pass nobody reads the grouped inputs again: the products overwrite them
-        ybuf = torch.empty(wide, dtype=torch.uint8, device=x.device) if train else None
-        y = ybuf.data_ptr() if train else sp["xs"]
-        _call(x, "kb_moe_experts_fwd", _p(x), x.stride(0), _p(weights), int(weights.dtype == torch.float32), _p(plan.offsets), _p(plan.slots),
-              _p(plan.rows), _p(plan.tiles), _p(wg), wg.stride(1), _stride0(wg), _p(wu), wu.stride(1), _stride0(wu), _p(wd), wd.stride(1), _stride0(wd),
-              _p(residual), residual.stride(0) if residual is not None else 0, _p(out), sp["xs"], sp["rw"], sp["g"], sp["u"], sp["h"], y, T, k, D, F, E, R)
-        _lib.add_launches(3)
-        if train:
-            ctx.save_for_backward(sp.buf, wg, wu, wd, *plan)
-            ctx.space, ctx.groups = sp.offset, groups
-            ctx.sizes = (T, k, D, F, E, R, weights.dtype, n_each)
-            for i, w in enumerate(ws):
-                if ctx.needs_input_grad[6 + i]:
-                    _count_use(w)
+        out, sp, stacks = _experts_forward(x, weights, residual, plan, groups, True)
+        ctx.save_for_backward(sp.buf, *stacks, plan.offsets, plan.slots, plan.rows, plan.tiles)
+        ctx.space, ctx.groups, ctx.n_each, ctx.w_dtype = sp.offset, groups, n_each, weights.dtype
+        for i, w in enumerate(ws):
+            if ctx.needs_input_grad[5 + i]:
+                _count_use(w)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        buf, wg, wu, wd, _, offsets, slots, rows, tiles = ctx.saved_tensors
-        T, k, D, F, E, R, w_dtype, n_each = ctx.sizes
+        buf, wg, wu, wd, offsets, slots, rows, tiles = ctx.saved_tensors
+        (T, k), (E, F, D), R, n_each, need = slots.view(-1, slots.shape[-1]).shape, wg.shape, rows.numel(), ctx.n_each, ctx.needs_input_grad
         at = {name: buf.data_ptr() + o for name, o in ctx.space.items()}
         dout = _rows2d(dout)
         dev = dout.device
-        need = ctx.needs_input_grad
-        n_part = 2 * -(-F // 256)
-        sp = _Space(dev, dys=2 * R * D, dg=2 * R * F, du=2 * R * F, part=4 * R * n_part)
+        sp = _Space(dev, dys=2 * R * D, dg=2 * R * F, du=2 * R * F, part=4 * R * 2 * -(-F // 256))
         dx = torch.empty((T, D), dtype=dout.dtype, device=dev) if need[0] else None
-        dw = torch.empty((T, k), dtype=w_dtype, device=dev) if need[1] else None
-        wants = [any(need[6 + i * n_each:6 + (i + 1) * n_each]) for i in range(3)]
-        mains = [_grad_view(g) for g in ctx.groups]
-        into = all(need[6:]) and all(m is not None for m in mains)
-        if into:
+        dw = torch.empty((T, k), dtype=ctx.w_dtype, device=dev) if need[1] else None
+        mains = [_grad_view(g) for g in ctx.groups] if all(need[5:]) else [None]
+        into = all(m is not None for m in mains)
+        if into:    # accumulate straight into the flat gradient buffer
             grads = mains
         else:
-            both = wants[0] or wants[1]
-            grads = [torch.empty((E, F, D), dtype=wg.dtype, device=dev) if both else None,
-                     torch.empty((E, F, D), dtype=wg.dtype, device=dev) if both else None,
-                     torch.empty((E, D, F), dtype=wg.dtype, device=dev) if wants[2] else None]
-        where = [v for g in grads for v in ((_p(g), g.stride(1), _stride0(g)) if g is not None else (None, 0, 0))]
-        _call(dout, "kb_moe_experts_bwd", _p(dout), dout.stride(0), at["xs"], at["rw"], at["g"], at["u"], at["h"], _p(offsets), _p(slots), _p(rows),
-              _p(tiles), _p(wg), wg.stride(1), _stride0(wg), _p(wu), wu.stride(1), _stride0(wu), _p(wd), wd.stride(1), _stride0(wd), sp["dys"], sp["dg"],
-              sp["du"], sp["part"], _p(dx), _p(dw), int(w_dtype == torch.float32), *where, int(into), T, k, D, F, E, R)
-        _lib.add_launches(1 + bool(grads[2] is not None) + bool(need[0]) + bool(need[0] or need[1]) + bool(grads[0] is not None))
+            gate_up, down = any(need[5:5 + 2 * n_each]), any(need[5 + 2 * n_each:])
+            grads = [torch.empty(w.shape, dtype=w.dtype, device=dev) if wanted else None for w, wanted in ((wg, gate_up), (wu, gate_up), (wd, down))]
+        where = [v for g in grads for v in (_where(g) if g is not None else (None, 0, 0))]
+        _call(dout, "kb_moe_experts_bwd", dout.data_ptr(), dout.stride(0), at["xs"], at["rw"], at["g"], at["u"], at["h"], offsets.data_ptr(),
+              slots.data_ptr(), rows.data_ptr(), tiles.data_ptr(), *_where(wg), *_where(wu), *_where(wd), sp["dys"], sp["dg"], sp["du"], sp["part"],
+              _p(dx), _p(dw), ctx.w_dtype == torch.float32, *where, into, T, k, D, F, E, R)
+        _lib.add_launches(1 + (grads[2] is not None) + (dx is not None) + (dx is not None or dw is not None) + (grads[0] is not None))
         out = []
         for i, group in enumerate(ctx.groups):
             if into:
@@ -376,26 +396,25 @@ class _ExpertsFn(torch.autograd.Function):
                     _use_done(w)
                 out += [None] * n_each
             else:
-                for j in range(n_each):
-                    wanted = need[6 + i * n_each + j]
-                    out.append((grads[i] if group[0].dim() == 3 else grads[i][j]) if wanted else None)
-        return (dx, dw, dout if need[2] else None, None, None, None, *out)
+                wanted = need[5 + i * n_each:5 + (i + 1) * n_each]
+                out += [(grads[i] if group[0].dim() == 3 else grads[i][j]) if wanted[j] else None for j in range(n_each)]
+        return (dx, dw, dout if need[2] else None, None, None, *out)
 
 
 def _experts_small(x, w, ids, res, wg, wu, wd) -> Tensor:
     (T, D), k, (E, F, _) = x.shape, w.shape[1], wg.shape
     out = torch.empty((T, D), dtype=x.dtype, device=x.device)
     h = torch.empty((T * k, F), dtype=torch.float32, device=x.device)
-    _call(x, "kb_moe_experts_small", _p(x), x.stride(0), _p(w), int(w.dtype == torch.float32), _p(ids), int(ids.dtype == torch.int64), _p(wg), wg.stride(1),
-          _stride0(wg), _p(wu), wu.stride(1), _stride0(wu), _p(wd), wd.stride(1), _stride0(wd), _p(res), res.stride(0) if res is not None else 0, _p(out), _p(h),
-          T, k, D, F, E)
+    _call(x, "kb_moe_experts_small", _p(x), x.stride(0), _p(w), int(w.dtype == torch.float32), _p(ids), int(ids.dtype == torch.int64), *_where(wg), *_where(wu),
+          *_where(wd), _p(res), 0 if res is None else res.stride(0), out.data_ptr(), h.data_ptr(), T, k, D, F, E)
     _lib.add_launches(1)
     return out
 
 
 def _rows2d(t: Tensor) -> Tensor:
     """``[rows, D]`` with unit inner stride and a pitch in multiples of 16 bytes."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else t.contiguous()
 
 
@@ -425,34 +444,45 @@ def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up
     The kernels take CUDA bf16 with D and F in multiples of 8 (weights also fp32); sums are held in fp32 and rounded once,
     the hidden activations and each expert's output row are bf16.
     """
-    stacks = [[w] if isinstance(w, Tensor) else list(w) for w in (w_gate, w_up, w_down)]
-    n_each = len(stacks[0])
     lone = isinstance(w_gate, Tensor)
-    shapes = [tuple(w.shape) if lone else (len(s), *s[0].shape) for s, w in zip(stacks, (w_gate, w_up, w_down)) if s]
-    if (len(shapes) < 3 or any(isinstance(w, Tensor) != lone for w in (w_gate, w_up, w_down)) or any(len(s) != 3 for s in shapes)
-            or shapes[1] != shapes[0] or shapes[2] != (shapes[0][0], shapes[0][2], shapes[0][1])
-            or any(w.shape != s[0].shape for s in stacks for w in s)):
+    if any(isinstance(w, Tensor) != lone for w in (w_up, w_down)):
+        raise ValueError("moe_experts: gate, up and down must all be stacked tensors or all be sequences of matrices")
+    if lone:
+        groups = ((w_gate,), (w_up,), (w_down,))
+        shapes = [tuple(w_gate.shape), tuple(w_up.shape), tuple(w_down.shape)]
+    else:
+        groups = tuple(tuple(w) for w in (w_gate, w_up, w_down))
+        shapes = [(len(g), *g[0].shape) if g and all(w.shape == g[0].shape for w in g) else () for g in groups]
+    if len(shapes[0]) != 3 or shapes[1] != shapes[0] or shapes[2] != (shapes[0][0], shapes[0][2], shapes[0][1]):
         raise ValueError(f"moe_experts: weights must be gate and up [E, F, D] and down [E, D, F], got {shapes}")
     E, F, D = shapes[0]
     _check_ids(experts, E, "moe_experts")
-    if x.dim() < 1 or x.shape[-1] != D or experts.shape[:-1] != x.shape[:-1] or weights.shape != experts.shape:
-        raise ValueError(f"moe_experts: x {tuple(x.shape)}, weights {tuple(weights.shape)}, experts {tuple(experts.shape)} do not fit [..., {D}], [..., k], [..., k]")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"moe_experts: residual {tuple(residual.shape)} has not the shape of x {tuple(x.shape)}")
-    k = experts.shape[-1]
-    every = [w for s in stacks for w in s]
-    if any(t.device != x.device for t in (weights, experts, *every, *([residual] if residual is not None else []))):
+    shape, ids_shape = x.shape, experts.shape
+    if not shape or shape[-1] != D or ids_shape[:-1] != shape[:-1] or weights.shape != ids_shape:
+        raise ValueError(f"moe_experts: x {tuple(shape)}, weights {tuple(weights.shape)}, experts {tuple(ids_shape)} do not fit [..., {D}], [..., k], [..., k]")
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"moe_experts: residual {tuple(residual.shape)} has not the shape of x {tuple(shape)}")
+    every = groups[0] + groups[1] + groups[2] + ((weights, x) if residual is None else (weights, x, residual))
+    if experts.device != x.device or any(t.device != x.device for t in every):
         raise ValueError("moe_experts: all tensors must be on one device")
-    if plan is not None and (plan.slots.shape != experts.shape or plan.counts.numel() != E or plan.rows.device != x.device):
+    if plan is not None and (plan.slots.shape != ids_shape or plan.counts.numel() != E or plan.rows.device != x.device):
         raise ValueError("moe_experts: the plan is not one of these experts")
-    x2, w2, ids2 = x.reshape(-1, D), weights.reshape(-1, k), experts.reshape(-1, k)
-    r2 = None if residual is None else residual.reshape(-1, D)
-    kernel = (x.is_cuda and x.dtype == torch.bfloat16 and all(w.dtype == torch.bfloat16 for w in every) and D % 8 == 0 and F % 8 == 0
-              and weights.dtype in (torch.bfloat16, torch.float32) and (r2 is None or r2.dtype == torch.bfloat16) and ids2.numel() > 0)
-    if not kernel:
-        return _experts_torch(x2, w2, ids2, *(s[0] if lone else s for s in stacks), r2).view(x.shape)
-    train = torch.is_grad_enabled() and any(t.requires_grad for t in (x2, w2, *every, *([r2] if r2 is not None else [])))
-    if not train and ids2.numel() <= SMALL:
-        return _experts_small(_rows2d(x2), w2.contiguous(), ids2.contiguous(), None if r2 is None else _rows2d(r2), *(_stacked(s) for s in stacks)).view(x.shape)
-    plan = moe_plan(ids2, E) if plan is None else plan
-    return _ExpertsFn.apply(_rows2d(x2), w2.contiguous(), None if r2 is None else _rows2d(r2), plan, n_each, train, *every).view(x.shape)
+    k = ids_shape[-1]
+    if len(shape) != 2:
+        x, weights, experts = x.reshape(-1, D), weights.reshape(-1, k), experts.reshape(-1, k)
+        residual = None if residual is None else residual.reshape(-1, D)
+    bf16 = torch.bfloat16
+    if (not x.is_cuda or D % 8 or F % 8 or experts.numel() == 0 or weights.dtype not in _KERNEL_DTYPES
+            or any(t.dtype != bf16 for t in every if t is not weights)):
+        return _experts_torch(x, weights, experts, *(g[0] if lone else g for g in groups), residual).view(shape)
+    train = torch.is_grad_enabled() and any(t.requires_grad for t in every)
+    x, weights, residual = _rows2d(x), weights.contiguous(), None if residual is None else _rows2d(residual)
+    if not train and experts.numel() <= SMALL:
+        out = _experts_small(x, weights, experts.contiguous(), residual, *(_stacked(g) for g in groups))
+    else:
+        plan = moe_plan(experts, E) if plan is None else plan
+        if train:
+            out = _ExpertsFn.apply(x, weights, residual, plan, len(groups[0]), *(w for g in groups for w in g))
+        else:
+            out = _experts_forward(x, weights, residual, plan, groups, False)[0]
+    return out if len(shape) == 2 else out.view(shape)
