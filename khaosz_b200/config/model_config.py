@@ -65,7 +65,11 @@ class AutoRegressiveLMConfig(BaseModelConfig):
     n_routed_experts: Optional[int] = None
     n_shared_experts: Optional[int] = None
     n_activated_experts: Optional[int] = None
-    topk_method: Optional[str] = None
+    topk_method: Optional[str] = None        # "softmax" / "sigmoid": fused routing and grouped experts
+    n_expert_groups: Optional[int] = None    # the rest with those two methods only
+    n_limited_groups: Optional[int] = None
+    router_bias: Optional[bool] = None
+    router_scale: Optional[float] = None
 
 
 @ConfigFactory.register("embedding")

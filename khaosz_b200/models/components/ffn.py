@@ -3,8 +3,10 @@
 Reference behaviour: ``astrai/model/components/mlp.py:16-93`` (``down(up(x) * silu(gate(x)))``,
 router softmax in fp32 -> top-k -> renormalise, shared experts averaged).  The MLP runs
 gate and up as one GEMM over adjacent weights with the SwiGLU in that GEMM's epilogue, and the
-down projection with the residual add in its epilogue.  The MoE dispatch is sort-based (one ``argsort``, no
-per-expert ``nonzero`` round trips to the host).
+down projection with the residual add in its epilogue.  The reference's MoE routing (``topk_method="greedy"``)
+dispatches with one ``argsort``, without per-expert ``nonzero`` round trips to the host; the other routing methods
+(``"softmax"``, ``"sigmoid"``) run on the fused routing and grouped expert kernels and never read a count on the host,
+so that training and decode steps can be recorded as CUDA graphs.
 """
 
 from __future__ import annotations
@@ -50,15 +52,38 @@ class MLP(nn.Module):
 
 @FFNFactory.register("moe")
 class DeepSeekMoE(nn.Module):
+    """Mixture of experts.  ``topk_method``:
+
+    * ``"greedy"`` (default, and any name not listed here): softmax in fp32, rounded to the activations' type, top-k, renormalised.
+    * ``"softmax"`` / ``"sigmoid"``: :func:`~khaosz_b200.ops.moe_route` with that score in fp32 and :func:`~khaosz_b200.ops.moe_experts`.
+      ``n_expert_groups`` / ``n_limited_groups`` restrict a token to the experts of its best groups, ``router_bias`` adds a buffer
+      ``[experts]`` to the scores for the selection only (balance the load by moving it between steps), ``router_scale`` scales
+      the renormalised weights.  The kernels read the experts' matrices in place from a packed model (``pack_parameters``, or any
+      executor's flat buffers) and from a copy otherwise.
+    """
+
+    FUSED = ("softmax", "sigmoid")
+
     def __init__(self, dim: int, dim_ffn: int, n_routed_experts: int, n_shared_experts: int = 1,
-                 n_activated_experts: int = 2, topk_method: str = "greedy"):
+                 n_activated_experts: int = 2, topk_method: str = "greedy", n_expert_groups: Optional[int] = None,
+                 n_limited_groups: Optional[int] = None, router_bias: Optional[bool] = None,
+                 router_scale: Optional[float] = None):
         super().__init__()
         self.dim = dim
         self.n_routed_experts = n_routed_experts
         self.n_shared_experts = n_shared_experts or 0
         self.n_activated_experts = n_activated_experts
         self.topk_method = topk_method
+        if topk_method not in self.FUSED and any(v is not None for v in (n_expert_groups, n_limited_groups, router_bias, router_scale)):
+            raise ValueError(f"expert groups, router_bias and router_scale need topk_method 'softmax' or 'sigmoid', not {topk_method!r}")
+        self.n_expert_groups = n_expert_groups or 1
+        self.n_limited_groups = n_limited_groups or self.n_expert_groups
+        self.router_scale = 1.0 if router_scale is None else float(router_scale)
         self.router = Linear(dim, n_routed_experts)
+        if router_bias:
+            self.register_buffer("router_bias", torch.zeros(n_routed_experts))
+        else:
+            self.router_bias = None
         self.shared_experts = nn.ModuleList(MLP(dim, dim_ffn) for _ in range(self.n_shared_experts))
         self.routed_experts = nn.ModuleList(MLP(dim, dim_ffn) for _ in range(n_routed_experts))
 
@@ -67,11 +92,39 @@ class DeepSeekMoE(nn.Module):
         weights, experts = torch.topk(probs, self.n_activated_experts, dim=-1)
         return weights / weights.sum(dim=-1, keepdim=True), experts
 
-    def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tensor:
-        shape = x.shape
-        flat = x.reshape(-1, shape[-1])
-        n_tok, k = flat.shape[0], self.n_activated_experts
-        weights, experts = self.route(flat)
+    def _expert_weights(self):
+        """The experts' gate, up and down matrices; ``None`` where a projection is not a plain Linear (adapters, int8)."""
+        stacks = []
+        for name in ("gate", "up", "down"):
+            mods = [e._modules[name] for e in self.routed_experts._modules.values()]
+            if any(type(m) is not Linear or m._parameters.get("bias") is not None for m in mods):
+                return None
+            stacks.append([m._parameters["weight"] for m in mods])
+        return stacks
+
+    def _router_logits(self, flat: Tensor) -> Tensor:
+        pad = -self.n_routed_experts % 8
+        if pad == 0 or type(self.router) is not Linear or not (flat.is_cuda and flat.dtype == torch.bfloat16):
+            return self.router(flat)
+        # the GEMM's rows are multiples of 16 bytes: surplus columns are computed and left out
+        return ops.linear(flat, nn.functional.pad(self.router.weight, (0, 0, 0, pad)))[:, :self.n_routed_experts]
+
+    def _forward_fused(self, flat: Tensor, residual: Optional[Tensor]) -> Tensor:
+        weights, experts = ops.moe_route(self._router_logits(flat), self.n_activated_experts, score=self.topk_method, bias=self.router_bias,
+                                         n_groups=self.n_expert_groups, topk_groups=self.n_limited_groups, scale=self.router_scale,
+                                         dtype=torch.float32)
+        if self.n_shared_experts == 1:
+            residual = self.shared_experts[0](flat, residual)
+        elif self.n_shared_experts:
+            shared = sum(e(flat) for e in self.shared_experts) / self.n_shared_experts
+            residual = shared if residual is None else residual + shared
+        stacks = self._expert_weights()
+        if stacks is not None:
+            return ops.moe_experts(flat, weights, experts, *stacks, residual=residual)
+        return self._expert_loop(flat, weights.to(flat.dtype), experts, residual)
+
+    def _expert_loop(self, flat: Tensor, weights: Tensor, experts: Tensor, residual: Optional[Tensor]) -> Tensor:
+        k = self.n_activated_experts
         # group the (token, slot) assignments by expert with one sort
         order = torch.argsort(experts.reshape(-1), stable=True)
         token_of = torch.div(order, k, rounding_mode="floor")
@@ -86,6 +139,15 @@ class DeepSeekMoE(nn.Module):
         out = torch.zeros_like(flat)
         if pieces:
             out.index_add_(0, token_of, torch.cat(pieces, dim=0) * w_sorted)
+        return out if residual is None else out + residual
+
+    def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tensor:
+        shape = x.shape
+        flat = x.reshape(-1, shape[-1])
+        if self.topk_method in self.FUSED:
+            return self._forward_fused(flat, None if residual is None else residual.reshape(-1, shape[-1])).view(shape)
+        weights, experts = self.route(flat)
+        out = self._expert_loop(flat, weights, experts, None)
         if self.n_shared_experts:
             out = out + sum(e(flat) for e in self.shared_experts) / self.n_shared_experts
         out = out.view(shape)

@@ -56,7 +56,8 @@ def _block_kwargs(cfg) -> Dict[str, Any]:
                      qk_rope_head_dim=cfg.qk_rope_head_dim)
     if getattr(cfg, "ffn_type", "mlp") == "moe":
         extra.update(n_routed_experts=cfg.n_routed_experts, n_shared_experts=cfg.n_shared_experts,
-                     n_activated_experts=cfg.n_activated_experts, topk_method=cfg.topk_method)
+                     n_activated_experts=cfg.n_activated_experts, topk_method=cfg.topk_method, n_expert_groups=cfg.n_expert_groups,
+                     n_limited_groups=cfg.n_limited_groups, router_bias=cfg.router_bias, router_scale=cfg.router_scale)
     return extra
 
 
