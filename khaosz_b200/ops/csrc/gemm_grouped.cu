@@ -16,6 +16,11 @@
 // 128 gate features and the same 128 up features, so SwiGLU, the routing weight and the rounding to bf16 happen
 // once, in the epilogue.  In the weight gradients K runs over an expert's rows in steps of 16, the alignment of
 // its segment, whose padding rows are zero.  All waits are bounded (common.cuh).
+//
+// Two forms.  A single CTA per tile reads (128 + 256) x 64 operands per K block: 92 bytes per clock at the tensor
+// cores' full rate, more than the about 64 that reach an SM from L2, and that bounds it (13 to 15 TB/s measured).
+// PAIR: two CTAs of a cluster compute 256 x 256 together (tcgen05 cta_group::2), each staging its own 128 rows
+// and half of B, 61 bytes per clock.  A pair's tile is wasted by experts with few rows, see use_pair().
 #include "common.cuh"
 #include "kb_api.h"
 #include "moe.cuh"
@@ -25,17 +30,22 @@ namespace grouped {
 
 enum Mode { GATE_UP = 0, DOWN = 1, DHID = 2, DX = 3, DW_DOWN = 4, DW_GU = 5 };
 
-constexpr int BM = KB_MOE_TILE_ROWS;
+constexpr int BM = KB_MOE_TILE_ROWS;  // rows per CTA
 constexpr int BN = 256;
 constexpr int BK = 64;
 constexpr int UMMA_K = 16;
-constexpr int STAGES = 4;
 constexpr int A_BYTES = BM * BK * 2;
-constexpr int B_BYTES = BN * BK * 2;
 constexpr int ATOM_BYTES = BK * 128;
-constexpr int SMEM_BYTES = STAGES * (A_BYTES + B_BYTES) + 256 + 1024;
-constexpr int EPI_WARPS = 8;  // two per TMEM lane quarter, each half of the columns
+constexpr int EPI_WARPS = 4;  // one per TMEM lane quarter (eight measured slower: GATE_UP 347 against 329 us)
 constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
+constexpr int STAGING = 32 * 128;  // DHID: bytes of one warp's 32 rows x 64 bf16, for each of its two operands
+template <int MODE, bool PAIR>
+struct Cfg {
+  static constexpr int B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2;
+  static constexpr int STAGES = PAIR ? (MODE == DHID ? 6 : 7) : 4;
+  static constexpr int STAGING_BYTES = MODE == DHID ? EPI_WARPS * 2 * STAGING : 0;
+  static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + STAGING_BYTES + 256 + 1024;
+};
 static_assert(BM == 128 && KB_MOE_ROW_ALIGN == UMMA_K, "a segment begins on a K step");
 
 struct Params {
@@ -48,7 +58,7 @@ struct Params {
   long ld0, ld1, stride0, stride1;  // pitch and (weight gradients) distance of the experts
   const __nv_bfloat16 *g, *u;       // DHID: [rows, N]
   const float* rw;                  // GATE_UP, DHID: routing weight of a row
-  float* part;                      // DHID: [rows, 2 num_n]
+  float* part;                      // DHID: [rows, num_n]
   int accumulate;                   // weight gradients: add to what is there
   int* err;
 };
@@ -59,33 +69,51 @@ struct Unit {
   int k0, klen;       // weight-gradient modes: first row and number of rows of the segment
 };
 
-template <int MODE>
-__device__ __forceinline__ Unit unit_of(const Params& p, int u) {
+// Work unit u of `total` -> row of tiles and first column.  In the row modes a last column of half tiles comes behind all
+// whole ones, so that the last, partly filled wave is made of short units (DHID 215 -> 200 us; in the weight gradients,
+// which would read an expert's rows a second time, it cost 3 %).
+template <int MODE, bool PAIR>
+__device__ __forceinline__ void column_of(const Params& p, int u, int total, int& x, int& n0) {
+  constexpr int WIDTH = MODE == GATE_UP ? BN / 2 : BN;
+  const int tail = MODE != GATE_UP && MODE < DW_DOWN && p.num_n > 1 && p.N - (p.num_n - 1) * BN <= BN / 2;
+  const int whole = p.num_n - tail, first_tail = total / p.num_n * whole;
+  if (u < first_tail) {
+    x = u / whole;
+    n0 = (u - x * whole) * WIDTH;
+  } else {
+    x = u - first_tail;
+    n0 = whole * WIDTH;
+  }
+}
+
+// What CTA `rank` of a pair (0 without pairs) does of work unit u.
+template <int MODE, bool PAIR>
+__device__ __forceinline__ Unit unit_of(const Params& p, int u, int total, int rank) {
   Unit r;
+  int x;  // row tile, or block of an expert's matrix
+  column_of<MODE, PAIR>(p, u, total, x, r.n0);
   if constexpr (MODE < DW_DOWN) {
-    const int m = u / p.num_n;
-    const int4 t = __ldg(p.tiles + 1 + m);
-    r.e = t.x; r.row0 = t.y; r.end = t.z;
-    r.n0 = (u - m * p.num_n) * (MODE == GATE_UP ? BN / 2 : BN);
+    const int4 t = __ldg(p.tiles + 1 + x);
+    r.e = t.x; r.row0 = t.y + (PAIR ? rank * BM : 0); r.end = t.z;
     r.m0 = r.mat = r.k0 = r.klen = 0;
   } else {
-    int x = u / p.num_n;
-    r.n0 = (u - x * p.num_n) * BN;
-    const int m = x % p.num_m;
-    x /= p.num_m;
-    r.m0 = m * BM;
-    if constexpr (MODE == DW_GU) { r.mat = x & 1; r.e = x >> 1; }
-    else { r.mat = 0; r.e = x; }
+    // the 128-row blocks of an expert's matrix, or of its two matrices one after the other; a pair takes two of them
+    const int blocks = MODE == DW_GU ? 2 * p.num_m : p.num_m, units = PAIR ? (blocks + 1) / 2 : blocks;
+    r.e = x / units;
+    const int m = (x - r.e * units) * (PAIR ? 2 : 1) + (PAIR ? rank : 0);
+    r.mat = MODE == DW_GU && m >= p.num_m;
+    r.m0 = (m - (r.mat ? p.num_m : 0)) * BM;
     r.k0 = __ldg(p.offsets + r.e);
     r.klen = __ldg(p.offsets + r.e + 1) - r.k0;
     r.row0 = r.end = 0;
   }
   return r;
 }
-template <int MODE>
+template <int MODE, bool PAIR>
 __device__ __forceinline__ int unit_count(const Params& p) {
   if constexpr (MODE < DW_DOWN) return __ldg(reinterpret_cast<const int*>(p.tiles)) * p.num_n;
-  else return p.E * (MODE == DW_GU ? 2 : 1) * p.num_m * p.num_n;
+  const int blocks = MODE == DW_GU ? 2 * p.num_m : p.num_m;
+  return p.E * (PAIR ? (blocks + 1) / 2 : blocks) * p.num_n;
 }
 template <int MODE>
 __device__ __forceinline__ int k_blocks(const Params& p, const Unit& t) {
@@ -93,11 +121,77 @@ __device__ __forceinline__ int k_blocks(const Params& p, const Unit& t) {
   else if constexpr (MODE == DX) return 2 * p.num_k;
   else return (t.klen + BK - 1) / BK;
 }
-
-// Columns of a tile that are computed: the last tile of a row stops at a multiple of 64.
-template <int MODE>
+// Columns of a tile that are computed: the last tile of a row stops at a multiple of 64 (a pair: of 128).
+template <int MODE, bool PAIR>
 __device__ __forceinline__ int tile_cols(const Params& p, const Unit& t) {
-  return MODE == GATE_UP ? BN : min(BN, (p.N - t.n0 + 63) / 64 * 64);
+  constexpr int STEP = PAIR ? 128 : 64;
+  return MODE == GATE_UP ? BN : min(BN, (p.N - t.n0 + STEP - 1) / STEP * STEP);
+}
+
+// ---- pairs of CTAs ------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t of_cta(uint32_t smem_addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same operation for a CTA alone and for a CTA of a pair.  A pair's loads land in the CTA that issues them and
+// count their bytes on the leader's barrier `bar` (no multicast); commits and arrivals name a barrier of the cluster.
+template <bool PAIR>
+__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+                 "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y)
+                 : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void load_3d(void* dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+                 "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    umma_f16(d, a, b, idesc, accumulate);
+}
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t* bar) {  // the barrier of every CTA of the pair
+  if constexpr (PAIR) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(of_cta(smem_u32(bar), r)) : "memory");
+  } else {
+    umma_commit(bar);
+  }
 }
 
 __device__ __forceinline__ uint4 pack8(const float* f) {
@@ -109,25 +203,31 @@ __device__ __forceinline__ void unpack8(const uint4& v, float* f) {
 }
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
-template <int MODE>
+template <int MODE, bool PAIR>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a2,
                const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_b2, const Params p) {
   constexpr bool A_MN = MODE >= DW_DOWN;
   constexpr bool B_MN = MODE >= DHID;
+  using C = Cfg<MODE, PAIR>;
+  constexpr int STAGES = C::STAGES;
+  constexpr int B_BYTES = C::B_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * A_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sB + STAGES * B_BYTES);
-  uint64_t* empty = full + STAGES;
-  uint64_t* tfull = empty + STAGES;
-  uint64_t* tempty = tfull + 2;
+  uint8_t* staging = sB + STAGES * B_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING_BYTES);  // (pairs: only the leader's are waited on)
+  uint64_t* empty = full + STAGES;                                      // each CTA waits on its own
+  uint64_t* tfull = empty + STAGES;                                     // each CTA waits on its own
+  uint64_t* tempty = tfull + 2;                                         // (pairs: only the leader's are waited on)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const int rank = PAIR ? (int)cluster_rank() : 0;
+  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < STAGES; ++i) {
@@ -136,59 +236,84 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], EPI_WARPS);
+      mbar_init(&tempty[i], (PAIR ? 2 : 1) * EPI_WARPS);
     }
     mbar_fence_init();
     tma_prefetch_desc(&tmap_a);
     tma_prefetch_desc(&tmap_b);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // both CTAs' barriers exist before anything crosses the pair
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   kb::moe::await_predecessor();
-  const int total = unit_count<MODE>(p);
+  const int total = unit_count<MODE, PAIR>(p);
 
   if (warp == 0) {
     // ------------------------------- TMA producer -------------------------------
     if (lane == 0) {
+      constexpr int ALL = PAIR ? BN / 128 : BN / 64;  // MN-major atoms of a whole tile's B in this CTA
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int un = blockIdx.x; un < total && ok; un += gridDim.x) {
-        const Unit t = unit_of<MODE>(p, un);
+      for (int un = first; un < total && ok; un += step) {
+        const Unit t = unit_of<MODE, PAIR>(p, un, total, rank);
         const int nk = k_blocks<MODE>(p, t);
-        const int atoms = tile_cols<MODE>(p, t) / 64;
-        const uint32_t bytes = A_BYTES + (B_MN ? atoms * ATOM_BYTES : B_BYTES);
+        const int cols = tile_cols<MODE, PAIR>(p, t);
+        const int atoms = cols / (PAIR ? 128 : 64);                    // of B, MN-major, in this CTA
+        const int n0 = PAIR && MODE != GATE_UP ? t.n0 + rank * (cols / 2) : t.n0;
+        const uint32_t bytes = (PAIR ? 2 : 1) * (A_BYTES + (B_MN ? atoms * ATOM_BYTES : B_BYTES));
         for (int kb = 0; kb < nk; ++kb) {
           if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, p.err, KB_ERR_TIMEOUT_EMPTY)) {
             ok = false;
             break;
           }
-          mbar_expect_tx(&full[s], bytes);
+          if (rank == 0) mbar_expect_tx(&full[s], bytes);
+          const uint32_t bar = PAIR ? of_cta(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
           uint8_t* a = sA + s * A_BYTES;
           uint8_t* b = sB + s * B_BYTES;
           if constexpr (MODE == GATE_UP) {
-            tma_load_2d(a, &tmap_a, &full[s], kb * BK, t.row0);
-            tma_load_3d(b, &tmap_b, &full[s], kb * BK, t.n0, t.e);
-            tma_load_3d(b + B_BYTES / 2, &tmap_b2, &full[s], kb * BK, t.n0, t.e);
+            load_2d<PAIR>(a, &tmap_a, bar, kb * BK, t.row0);
+            if constexpr (PAIR) {  // one CTA stages the gate rows, the other the same features' up rows
+              load_3d<PAIR>(b, rank ? &tmap_b2 : &tmap_b, bar, kb * BK, n0, t.e);
+            } else {
+              load_3d<PAIR>(b, &tmap_b, bar, kb * BK, n0, t.e);
+              load_3d<PAIR>(b + B_BYTES / 2, &tmap_b2, bar, kb * BK, n0, t.e);
+            }
           } else if constexpr (MODE == DOWN) {
-            tma_load_2d(a, &tmap_a, &full[s], kb * BK, t.row0);
-            tma_load_3d(b, &tmap_b, &full[s], kb * BK, t.n0, t.e);
+            load_2d<PAIR>(a, &tmap_a, bar, kb * BK, t.row0);
+            load_3d<PAIR>(b, &tmap_b, bar, kb * BK, n0, t.e);
           } else if constexpr (MODE == DHID || MODE == DX) {
             const bool second = MODE == DX && kb >= p.num_k;
             const int k = (second ? kb - p.num_k : kb) * BK;
-            tma_load_2d(a, second ? &tmap_a2 : &tmap_a, &full[s], k, t.row0);
-            for (int i = 0; i < atoms; ++i) tma_load_3d(b + i * ATOM_BYTES, second ? &tmap_b2 : &tmap_b, &full[s], t.n0 + i * 64, k, t.e);
+            load_2d<PAIR>(a, second ? &tmap_a2 : &tmap_a, bar, k, t.row0);
+            const CUtensorMap* mb = second ? &tmap_b2 : &tmap_b;
+            if (atoms == ALL) {  // unrolled: the issuing thread is on the critical path (6 to 8 % of the kernel)
+#pragma unroll
+              for (int i = 0; i < ALL; ++i) load_3d<PAIR>(b + i * ATOM_BYTES, mb, bar, n0 + i * 64, k, t.e);
+            } else {
+              for (int i = 0; i < atoms; ++i) load_3d<PAIR>(b + i * ATOM_BYTES, mb, bar, n0 + i * 64, k, t.e);
+            }
           } else {
             const int k = t.k0 + kb * BK;
 #pragma unroll
-            for (int i = 0; i < BM / 64; ++i) tma_load_2d(a + i * ATOM_BYTES, t.mat ? &tmap_a2 : &tmap_a, &full[s], t.m0 + i * 64, k);
-            for (int i = 0; i < atoms; ++i) tma_load_2d(b + i * ATOM_BYTES, &tmap_b, &full[s], t.n0 + i * 64, k);
+            for (int i = 0; i < BM / 64; ++i) load_2d<PAIR>(a + i * ATOM_BYTES, t.mat ? &tmap_a2 : &tmap_a, bar, t.m0 + i * 64, k);
+            if (atoms == ALL) {
+#pragma unroll
+              for (int i = 0; i < ALL; ++i) load_2d<PAIR>(b + i * ATOM_BYTES, &tmap_b, bar, n0 + i * 64, k);
+            } else {
+              for (int i = 0; i < atoms; ++i) load_2d<PAIR>(b + i * ATOM_BYTES, &tmap_b, bar, n0 + i * 64, k);
+            }
           }
           if (++s == STAGES) {
             s = 0;
@@ -198,19 +323,19 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       }
     }
   } else if (warp == 1) {
-    // ------------------------------- MMA issuer -------------------------------
-    if (lane == 0) {
+    // ------------------------------- MMA issuer (the leader's) -------------------------------
+    if (lane == 0 && rank == 0) {
       int s = 0;
       uint32_t ph = 0;
       int acc = 0;
       uint32_t aph = 0;
       bool ok = true;
-      for (int un = blockIdx.x; un < total && ok; un += gridDim.x) {
+      for (int un = first; un < total && ok; un += step) {
         Unit t{};
-        if constexpr (MODE >= DW_DOWN) t = unit_of<MODE>(p, un);
-        else t.n0 = un % p.num_n * (MODE == GATE_UP ? BN / 2 : BN);
+        if constexpr (MODE >= DW_DOWN) t = unit_of<MODE, PAIR>(p, un, total, 0);
+        else column_of<MODE, PAIR>(p, un, total, t.row0, t.n0);
         const int nk = k_blocks<MODE>(p, t);
-        const uint32_t idesc = umma_idesc(BM, tile_cols<MODE>(p, t), A_MN, B_MN);
+        const uint32_t idesc = umma_idesc((PAIR ? 2 : 1) * BM, tile_cols<MODE, PAIR>(p, t), A_MN, B_MN);
         if (nk == 0) continue;  // an expert without rows: the epilogue writes zeros
         if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, p.err, KB_ERR_TIMEOUT_TMEM_EMPTY)) {
           ok = false;
@@ -230,19 +355,19 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           const int steps = MODE >= DW_DOWN ? min(BK, t.klen - kb * BK) / UMMA_K : BK / UMMA_K;
 #pragma unroll
           for (int j = 0; j < BK / UMMA_K; ++j) {
-            if (j >= steps) break;
+            if (MODE >= DW_DOWN && j >= steps) break;
             const uint64_t a_desc = A_MN ? umma_desc_mnmajor(a_addr, j * UMMA_K, ATOM_BYTES) : umma_desc_kmajor(a_addr, j * UMMA_K * 2);
             const uint64_t b_desc = B_MN ? umma_desc_mnmajor(b_addr, j * UMMA_K, ATOM_BYTES) : umma_desc_kmajor(b_addr, j * UMMA_K * 2);
-            umma_f16(d_tmem, a_desc, b_desc, idesc, (kb || j) ? 1u : 0u);
+            mma<PAIR>(d_tmem, a_desc, b_desc, idesc, (kb || j) ? 1u : 0u);
           }
-          umma_commit(&empty[s]);
+          commit<PAIR>(&empty[s]);
           if (++s == STAGES) {
             s = 0;
             ph ^= 1u;
           }
         }
         if (!ok) break;
-        umma_commit(&tfull[acc]);
+        commit<PAIR>(&tfull[acc]);
         if (++acc == 2) {
           acc = 0;
           aph ^= 1u;
@@ -252,16 +377,37 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   } else {
     // ------------------------------- epilogue -------------------------------
     const int q = warp & 3;  // TMEM lane quarter this warp may read
-    const int half = (warp - 2) >> 2;
     const int row = q * 32 + lane;
     int acc = 0;
     uint32_t aph = 0;
-    for (int un = blockIdx.x; un < total; un += gridDim.x) {
-      const Unit t = unit_of<MODE>(p, un);
+    for (int un = first; un < total; un += step) {
+      const Unit t = unit_of<MODE, PAIR>(p, un, total, rank);
       const bool any_k = k_blocks<MODE>(p, t) > 0;
       float w = 0.f;
       if constexpr (MODE == GATE_UP || MODE == DHID)
         if (t.row0 + row < t.end) w = p.rw[t.row0 + row];
+      // DHID: G and U come and dG and dU go in whole lines, eight lanes to a row's 64 columns, through the warp's own
+      // staging rows (16-byte pieces swizzled by the row); a lane that walked its own row would touch 32 lines per
+      // access, which held the tensor cores up (the kernel took 241 us so, now 215, of a main loop of 150).
+      uint8_t* sg = staging + (warp - 2) * 2 * STAGING;
+      uint8_t* su = sg + STAGING;
+      const int r8 = lane >> 3, c8 = lane & 7;
+      const size_t row0 = t.row0 + q * 32;
+      const int rows = min(32, t.end - (t.row0 + q * 32));
+      uint4 vg[8], vu[8];
+      auto fetch = [&](int c) {
+        const int col = t.n0 + c * 64 + c8 * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + r8;
+          vg[i] = vu[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < rows && col < p.N) {
+            vg[i] = *reinterpret_cast<const uint4*>(p.g + (row0 + r) * p.ld0 + col);
+            vu[i] = *reinterpret_cast<const uint4*>(p.u + (row0 + r) * p.ld0 + col);
+          }
+        }
+      };
+      if constexpr (MODE == DHID) fetch(0);
       if (any_k && !mbar_wait(&tfull[acc], aph, abort_flag, p.err, KB_ERR_TIMEOUT_TMEM_FULL)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
@@ -271,7 +417,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           const size_t grow = t.row0 + row;
           if constexpr (MODE == GATE_UP) {
 #pragma unroll 1
-            for (int c = half * (BN / 128); c < (half + 1) * (BN / 128); ++c) {
+            for (int c = 0; c < BN / 64; ++c) {
               const int col = t.n0 + c * 32;
               if (col >= p.N) break;
               uint32_t vg[32], vu[32];
@@ -299,27 +445,28 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           } else if constexpr (MODE == DHID) {
             float dot = 0.f;
 #pragma unroll 1
-            for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
-              const int col = t.n0 + c * 32;
-              if (col >= p.N) break;
-              uint4 vg[4], vu[4];
+            for (int c = 0; c < BN / 64; ++c) {
+              if (t.n0 + c * 64 >= p.N) break;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                vg[i] = vu[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (live && col + i * 8 < p.N) {
-                  vg[i] = *reinterpret_cast<const uint4*>(p.g + grow * p.ld0 + col + i * 8);
-                  vu[i] = *reinterpret_cast<const uint4*>(p.u + grow * p.ld0 + col + i * 8);
-                }
+              for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + r8;
+                *reinterpret_cast<uint4*>(sg + sw128_offset(r, c8)) = vg[i];
+                *reinterpret_cast<uint4*>(su + sw128_offset(r, c8)) = vu[i];
               }
-              uint32_t v[32];
-              tmem_ld_32x32b_x32(t_row + c * 32, v);
-              tmem_ld_wait();
+              __syncwarp();
+              if (c + 1 < BN / 64 && t.n0 + (c + 1) * 64 < p.N) fetch(c + 1);  // under way during the arithmetic
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float g[8], u[8], dg[8], du[8];
-                unpack8(vg[i], g);
-                unpack8(vu[i], u);
-                if (live && col + i * 8 < p.N) {
+              for (int h = 0; h < 2; ++h) {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(t_row + c * 64 + h * 32, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  uint4* pg = reinterpret_cast<uint4*>(sg + sw128_offset(lane, h * 4 + i));
+                  uint4* pu = reinterpret_cast<uint4*>(su + sw128_offset(lane, h * 4 + i));
+                  float g[8], u[8], dg[8], du[8];
+                  unpack8(*pg, g);
+                  unpack8(*pu, u);
 #pragma unroll
                   for (int x = 0; x < 8; ++x) {
                     const float d = __uint_as_float(v[i * 8 + x]), s = sigmoid(g[x]), act = g[x] * s;
@@ -327,15 +474,26 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                     dg[x] = w * d * u[x] * (s + act * (1.f - s));
                     du[x] = w * d * act;
                   }
-                  *reinterpret_cast<uint4*>(p.out0 + grow * p.ld0 + col + i * 8) = pack8(dg);
-                  *reinterpret_cast<uint4*>(p.out1 + grow * p.ld0 + col + i * 8) = pack8(du);
+                  *pg = pack8(dg);
+                  *pu = pack8(du);
                 }
               }
+              __syncwarp();
+              const int col = t.n0 + c * 64 + c8 * 8;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + r8;
+                if (r < rows && col < p.N) {
+                  *reinterpret_cast<uint4*>(p.out0 + (row0 + r) * p.ld0 + col) = *reinterpret_cast<const uint4*>(sg + sw128_offset(r, c8));
+                  *reinterpret_cast<uint4*>(p.out1 + (row0 + r) * p.ld0 + col) = *reinterpret_cast<const uint4*>(su + sw128_offset(r, c8));
+                }
+              }
+              __syncwarp();
             }
-            if (live) p.part[(grow * p.num_n + t.n0 / BN) * 2 + half] = dot;
+            if (live) p.part[grow * p.num_n + t.n0 / BN] = dot;
           } else {
 #pragma unroll 1
-            for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
+            for (int c = 0; c < BN / 32; ++c) {
               const int col = t.n0 + c * 32;
               if (col >= p.N) break;
               uint32_t v[32];
@@ -353,7 +511,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         __nv_bfloat16* o = t.mat ? p.out1 + t.e * p.stride1 + m * p.ld1 : p.out0 + t.e * p.stride0 + m * p.ld0;
         if (any_k || !p.accumulate) {
 #pragma unroll 1
-          for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
+          for (int c = 0; c < BN / 32; ++c) {
             const int col = t.n0 + c * 32;
             if (col >= p.N) break;
             uint32_t v[32];
@@ -385,7 +543,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       if (any_k) {  // accumulator fully read: hand it back to the MMA warp
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&tempty[acc]);
+        if (lane == 0) {
+          if constexpr (PAIR) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(of_cta(smem_u32(&tempty[acc]), 0)) : "memory");
+          else mbar_arrive(&tempty[acc]);
+        }
         if (++acc == 2) {
           acc = 0;
           aph ^= 1u;
@@ -396,9 +557,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // nothing of the pair touches the other CTA behind this point
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    else tmem_dealloc(tmem_base, 512);
   }
 }
 
@@ -417,16 +580,23 @@ static int weight_map(CUtensorMap* m, const Weight& w, int E, int rows, int cols
   return make_tmap_3d(m, w.p, 2, dims, strides, box, true) ? KB_STATUS_TMAP_ERROR : KB_STATUS_OK;
 }
 
-template <int MODE>
-static int launch(const CUtensorMap& a, const CUtensorMap& a2, const CUtensorMap& b, const CUtensorMap& b2, const Params& p, int dev, int grid,
-                  cudaStream_t st) {
+template <int MODE, bool PAIR>
+static int launch_form(const CUtensorMap& a, const CUtensorMap& a2, const CUtensorMap& b, const CUtensorMap& b2, const Params& p, int dev, int sms,
+                       cudaStream_t st) {
   static bool set[64] = {false};  // the attribute is per device
   if (!set[dev & 63]) {
-    if (cudaFuncSetAttribute(grouped_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return KB_STATUS_CUDA_ERROR;
+    if (cudaFuncSetAttribute(grouped_kernel<MODE, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<MODE, PAIR>::SMEM) != cudaSuccess)
+      return KB_STATUS_CUDA_ERROR;
     set[dev & 63] = true;
   }
-  return kb::moe::launch_after(grouped_kernel<MODE>, grid, NUM_THREADS, SMEM_BYTES, st, a, a2, b, b2, p) == cudaSuccess ? KB_STATUS_OK
-                                                                                                                         : KB_STATUS_CUDA_ERROR;
+  const cudaError_t e = PAIR ? kb::moe::launch_after<2>(grouped_kernel<MODE, PAIR>, sms / 2 * 2, NUM_THREADS, Cfg<MODE, PAIR>::SMEM, st, a, a2, b, b2, p)
+                             : kb::moe::launch_after(grouped_kernel<MODE, PAIR>, sms, NUM_THREADS, Cfg<MODE, PAIR>::SMEM, st, a, a2, b, b2, p);
+  return e == cudaSuccess ? KB_STATUS_OK : KB_STATUS_CUDA_ERROR;
+}
+template <int MODE>
+static int launch(bool pair, const CUtensorMap& a, const CUtensorMap& a2, const CUtensorMap& b, const CUtensorMap& b2, const Params& p, int dev, int sms,
+                  cudaStream_t st) {
+  return pair ? launch_form<MODE, true>(a, a2, b, b2, p, dev, sms, st) : launch_form<MODE, false>(a, a2, b, b2, p, dev, sms, st);
 }
 
 static int cdiv(int a, int b) { return (a + b - 1) / b; }
@@ -465,7 +635,7 @@ static int moe_sizes(int T, int k, int D, int F, int E, int R) {
 }
 
 extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, int w_f32, const int* offsets, const int* slots, const int* rows,
-                                  const int* tiles, const void* wg, long ldg, long sg, const void* wu, long ldu, long su, const void* wd, long ldd,
+                                  const int* tiles, int pair, const void* wg, long ldg, long sg, const void* wu, long ldu, long su, const void* wd, long ldd,
                                   long sd, const void* res, long ldr, void* out, void* xs, float* rw, void* g, void* u, void* h, void* y, int T, int k,
                                   int D, int F, int E, int R, void* stream) {
   using namespace kb::grouped;
@@ -495,21 +665,21 @@ extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, 
   p.out2 = static_cast<__nv_bfloat16*>(h);
   p.ld0 = F;
   p.rw = rw;
-  KB_TRY(launch<GATE_UP>(a, a, b, b2, p, d.dev, d.sms, st));
+  KB_TRY(launch<GATE_UP>(pair, a, a, b, b2, p, d.dev, d.sms, st));
   KB_TRY(rows_map(&a, h, R, F, BM));
-  KB_TRY(weight_map(&b, W, E, D, F, BN));
+  KB_TRY(weight_map(&b, W, E, D, F, pair ? BN / 2 : BN));
   p.num_n = cdiv(D, BN);
   p.num_k = cdiv(F, BK);
   p.N = D;
   p.out0 = static_cast<__nv_bfloat16*>(y);
   p.out1 = p.out2 = nullptr;
   p.ld0 = D;
-  KB_TRY(launch<DOWN>(a, a, b, b, p, d.dev, d.sms, st));
+  KB_TRY(launch<DOWN>(pair, a, a, b, b, p, d.dev, d.sms, st));
   return kb::moe::launch_combine(y, slots, res, ldr, out, nullptr, 0, nullptr, 0, T, k, D, st);
 }
 
 extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, const float* rw, const void* g, const void* u, const void* h,
-                                  const int* offsets, const int* slots, const int* rows, const int* tiles, const void* wg, long ldg, long sg,
+                                  const int* offsets, const int* slots, const int* rows, const int* tiles, int pair, const void* wg, long ldg, long sg,
                                   const void* wu, long ldu, long su, const void* wd, long ldd, long sd, void* dys, void* dg, void* du, float* part,
                                   void* dx, void* dw, int w_f32, void* dwg, long ldwg, long sdwg, void* dwu, long ldwu, long sdwu, void* dwd, long ldwd,
                                   long sdwd, int accumulate, int T, int k, int D, int F, int E, int R, void* stream) {
@@ -532,10 +702,10 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
   p.E = E;
   p.err = d.err;
   // dG, dU and the routing weights' partial gradients
-  const int n_part = 2 * cdiv(F, BN);
+  const int n_part = cdiv(F, BN);
   KB_TRY(rows_map(&a, dys, R, D, BM));
   KB_TRY(weight_map(&b, W, E, D, F, BK));
-  p.num_n = cdiv(F, BN);
+  p.num_n = n_part;
   p.num_k = cdiv(D, BK);
   p.N = F;
   p.out0 = static_cast<__nv_bfloat16*>(dg);
@@ -545,7 +715,7 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
   p.u = static_cast<const __nv_bfloat16*>(u);
   p.rw = rw;
   p.part = part;
-  KB_TRY(launch<DHID>(a, a, b, b, p, d.dev, d.sms, st));
+  KB_TRY(launch<DHID>(pair, a, a, b, b, p, d.dev, d.sms, st));
   p.g = p.u = nullptr;
   p.part = nullptr;
   p.accumulate = accumulate;
@@ -559,7 +729,7 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
     p.out0 = static_cast<__nv_bfloat16*>(dwd);
     p.ld0 = ldwd;
     p.stride0 = sdwd;
-    KB_TRY(launch<DW_DOWN>(a, a, b, b, p, d.dev, d.sms, st));
+    KB_TRY(launch<DW_DOWN>(pair, a, a, b, b, p, d.dev, d.sms, st));
   }
   if (dx) {
     KB_TRY(rows_map(&a, dg, R, F, BM));
@@ -571,7 +741,7 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
     p.N = D;
     p.out0 = static_cast<__nv_bfloat16*>(dys);
     p.ld0 = D;
-    KB_TRY(launch<DX>(a, a2, b, b2, p, d.dev, d.sms, st));
+    KB_TRY(launch<DX>(pair, a, a2, b, b2, p, d.dev, d.sms, st));
   }
   if (dx || dw) KB_TRY(kb::moe::launch_combine(dys, slots, nullptr, 0, dx, part, n_part, dw, w_f32, T, k, D, st));
   if (dwg) {
@@ -588,7 +758,7 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
     p.out1 = static_cast<__nv_bfloat16*>(dwu);
     p.ld1 = ldwu;
     p.stride1 = sdwu;
-    KB_TRY(launch<DW_GU>(a, a2, b, b, p, d.dev, d.sms, st));
+    KB_TRY(launch<DW_GU>(pair, a, a2, b, b, p, d.dev, d.sms, st));
   }
   return KB_STATUS_OK;
 }

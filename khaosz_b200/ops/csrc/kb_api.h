@@ -213,14 +213,14 @@ int kb_moe_route_fwd(const void* z, int z_f32, long ldz, const float* bias, void
 int kb_moe_route_bwd(const void* z, int z_f32, long ldz, const float* bias, const long long* ids, const void* dw, int w_f32, void* dz,
                      int T, int E, int k, int sigmoid, int renorm, float scale, void* stream);
 // Grouping of n assignments by expert.  counts [E], offsets [E+1], slots [n], rows [R], tiles [1 + tiles][4] (16-byte aligned,
-// R / 128 + min(E, n) tiles at most); R >= n + 15 min(E, n) rounded up to 16; hist [ceil(n / 2048), E] scratch (n > 2048).
+// R / 128 + min(E, n) tiles at most), pairs: the same of 256 rows (R / 256 + min(E, n)); R >= n + 15 min(E, n) rounded up to 16; hist [ceil(n / 2048), E] scratch (n > 2048).
 // An index outside 0..E-1 is dropped (slot -1).
-int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int* counts, int* offsets, int* slots, int* rows, int* tiles, int* hist,
-                void* stream);
-// out = res + the experts' products; the plan's arrays, the weights [E, F, D], [E, F, D], [E, D, F] (pitch, distance of the experts),
+int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int* counts, int* offsets, int* slots, int* rows, int* tiles, int* pairs,
+                int* hist, void* stream);
+// out = res + the experts' products; the plan's arrays (tiles: its tiles, or with `pair` its pairs, which two CTAs share), the weights [E, F, D], [E, F, D], [E, D, F] (pitch, distance of the experts),
 // and scratch: xs [R,D], rw [R], h [R,F], y [R,D] (may be xs); g, u [R,F] (both or neither) keep the projections for the backward pass.
 int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, int w_f32, const int* offsets, const int* slots, const int* rows,
-                       const int* tiles, const void* wg, long ldg, long sg, const void* wu, long ldu, long su, const void* wd, long ldd, long sd,
+                       const int* tiles, int pair, const void* wg, long ldg, long sg, const void* wu, long ldu, long su, const void* wd, long ldd, long sd,
                        const void* res, long ldr, void* out, void* xs, float* rw, void* g, void* u, void* h, void* y, int T, int k, int D, int F,
                        int E, int R, void* stream);
 // The same product for T * k <= KB_MOE_SMALL_MAX assignments, straight from the experts' indices (no plan); h [T*k, F] fp32 scratch.
@@ -228,9 +228,9 @@ int kb_moe_experts_small(const void* x, long ldx, const void* weights, int w_f32
                          const void* wu, long ldu, long su, const void* wd, long ldd, long sd, const void* res, long ldr, void* out, float* h,
                          int T, int k, int D, int F, int E, void* stream);
 // Backward pass: dx [T,D], dw [T,k] and the weights' gradients, each optional (dwg and dwu together); accumulate: the weights' gradients are
-// added to what is there.  Scratch: dys [R,D], dg, du [R,F], part [R, 2 ceil(F / 256)].
+// added to what is there.  Scratch: dys [R,D], dg, du [R,F], part [R, ceil(F / 256)].
 int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, const float* rw, const void* g, const void* u, const void* h,
-                       const int* offsets, const int* slots, const int* rows, const int* tiles, const void* wg, long ldg, long sg, const void* wu,
+                       const int* offsets, const int* slots, const int* rows, const int* tiles, int pair, const void* wg, long ldg, long sg, const void* wu,
                        long ldu, long su, const void* wd, long ldd, long sd, void* dys, void* dg, void* du, float* part, void* dx, void* dw,
                        int w_f32, void* dwg, long ldwg, long sdwg, void* dwu, long ldwu, long sdwu, void* dwd, long ldwd, long sdwd,
                        int accumulate, int T, int k, int D, int F, int E, int R, void* stream);

@@ -370,6 +370,7 @@ struct PlanParams {
   int* slots;     // [n]
   int* rows;      // [R]
   int4* tiles;    // [1 + max]: .x of the first = number of 128-row tiles, then (expert, first row, end row, 0)
+  int4* pairs;    // the same of 256 rows
   int* hist;      // [nb, E] (several blocks only)
 };
 
@@ -395,21 +396,28 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_count_kernel(const PlanPara
   for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS) p.hist[(size_t)blockIdx.x * p.E + e] = h[e];
 }
 
-// Exclusive prefix of two values per thread over the block.
-__device__ __forceinline__ void block_prefix2(int& a, int& b, int (*red)[2]) {
+// Exclusive prefix of N values per thread over the block.
+template <int N>
+__device__ __forceinline__ void block_prefix(int (&v)[N], int (*red)[N]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = a, y = b;
+  int x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = v[i];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(FULL, x, o), v = __shfl_up_sync(FULL, y, o);
-    if (lane >= o) { x += u; y += v; }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int u = __shfl_up_sync(FULL, x[i], o);
+      if (lane >= o) x[i] += u;
+    }
   }
-  if (lane == 31) { red[warp][0] = x; red[warp][1] = y; }
+  if (lane == 31) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[warp][i] = x[i];
+  }
   __syncthreads();
-  int bx = 0, by = 0;
-  for (int w = 0; w < warp; ++w) { bx += red[w][0]; by += red[w][1]; }
-  a = x - a + bx;
-  b = y - b + by;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = x[i] - v[i] + __reduce_add_sync(FULL, lane < warp ? red[lane][i] : 0);
 }
 
 // SINGLE: one block holds all assignments and nothing was counted before.
@@ -417,7 +425,7 @@ template <bool SINGLE>
 __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanParams p) {
   extern __shared__ uint16_t wc[];  // [32 warps][E]
   __shared__ int start[1024];       // first row of this block's assignments of an expert
-  __shared__ int red[32][2];
+  __shared__ int red[32][3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint16_t* mine = wc + warp * p.E;
   await_predecessor();
@@ -471,18 +479,22 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
   if (tid >= p.E) total = 0;
   const int padded = (total + ALIGN - 1) / ALIGN * ALIGN;
   const int tiles = (padded + TILE - 1) / TILE;
-  int off = padded, first = tiles;
-  block_prefix2(off, first, red);
+  const int pairs = (tiles + 1) / 2;
+  int begin[3] = {padded, tiles, pairs};
+  block_prefix(begin, red);
+  const int off = begin[0];
   if (tid < p.E) start[tid] = off + before;
   __syncthreads();
   if (blockIdx.x == 0) {
     if (tid < p.E) {
       p.counts[tid] = total;
       p.offsets[tid] = off;
-      for (int i = 0; i < tiles; ++i) p.tiles[1 + first + i] = make_int4(tid, off + i * TILE, off + padded, 0);
+      for (int i = 0; i < tiles; ++i) p.tiles[1 + begin[1] + i] = make_int4(tid, off + i * TILE, off + padded, 0);
+      for (int i = 0; i < pairs; ++i) p.pairs[1 + begin[2] + i] = make_int4(tid, off + 2 * i * TILE, off + padded, 0);
       if (tid == p.E - 1) {
         p.offsets[p.E] = off + padded;
-        p.tiles[0] = make_int4(first + tiles, 0, 0, 0);
+        p.tiles[0] = make_int4(begin[1] + tiles, 0, 0, 0);
+        p.pairs[0] = make_int4(begin[2] + pairs, 0, 0, 0);
       }
     }
   }
@@ -634,15 +646,15 @@ extern "C" int kb_moe_route_bwd(const void* z, int z_f32, long ldz, const float*
   return launched();
 }
 
-extern "C" int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int* counts, int* offsets, int* slots, int* rows, int* tiles, int* hist,
-                           void* stream) {
+extern "C" int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int* counts, int* offsets, int* slots, int* rows, int* tiles, int* pairs,
+                           int* hist, void* stream) {
   if (n < 1 || E < 1) return KB_STATUS_BAD_ARG;
   if (E > KB_MOE_MAX_EXPERTS || n > (1 << 30)) return KB_STATUS_TOO_LARGE;
   const int least = (n + (ALIGN - 1) * (E < n ? E : n) + ALIGN - 1) / ALIGN * ALIGN;
-  if (R < least || (reinterpret_cast<uintptr_t>(tiles) & 15)) return KB_STATUS_BAD_ARG;
+  if (R < least || ((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(pairs)) & 15)) return KB_STATUS_BAD_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int nb = (n + CHUNK - 1) / CHUNK;
-  PlanParams p{ids, ids64, n, E, R, nb, counts, offsets, slots, rows, reinterpret_cast<int4*>(tiles), hist};
+  PlanParams p{ids, ids64, n, E, R, nb, counts, offsets, slots, rows, reinterpret_cast<int4*>(tiles), reinterpret_cast<int4*>(pairs), hist};
   const int smem = 32 * E * 2;
   if (nb == 1) {
     if (smem > 32 * 1024 && cudaFuncSetAttribute(plan_place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)

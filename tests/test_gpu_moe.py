@@ -102,10 +102,10 @@ def test_plan(T, k, E, dtype):
     counts, offsets, slots, rows = plan_ref(ids, E)
     assert p.counts.tolist() == counts and p.offsets.tolist() == offsets
     assert p.slots.reshape(-1).tolist() == slots and p.rows.tolist() == rows
-    n_tiles = int(p.tiles[0, 0])
-    assert n_tiles + 1 <= p.tiles.shape[0]
-    want = [[e, r, offsets[e + 1], 0] for e in range(E) for r in range(offsets[e], offsets[e + 1], 128)]
-    assert p.tiles[1:1 + n_tiles].tolist() == want
+    for tiles, size in ((p.tiles, 128), (p.pairs, 256)):
+        n_tiles = int(tiles[0, 0])
+        assert n_tiles + 1 <= tiles.shape[0]
+        assert tiles[1:1 + n_tiles].tolist() == [[e, r, offsets[e + 1], 0] for e in range(E) for r in range(offsets[e], offsets[e + 1], size)]
     assert all(torch.equal(a, b) for a, b in zip(p[:4], again[:4]))
 
 
@@ -135,6 +135,14 @@ def _inputs(T, D, F, E, k, drop, seed=0):
     return x, w, ids, ws, res, dout
 
 
+@pytest.fixture(params=["one CTA", "pairs"])
+def form(request, monkeypatch):
+    """Both forms of the grouped products, whatever the rule between them says of the sizes."""
+    from khaosz_b200.ops import moe
+
+    monkeypatch.setattr(moe, "_use_pairs", lambda n, E: request.param == "pairs")
+
+
 def _check(got, ref, names, dtypes=None):
     for n in names:
         bad = outside(got[n], *ref[n], dtype=(dtypes or {}).get(n, torch.bfloat16))
@@ -142,7 +150,7 @@ def _check(got, ref, names, dtypes=None):
 
 
 @pytest.mark.parametrize("T,D,F,E,k,drop", SIZES)
-def test_experts_forward(T, D, F, E, k, drop):
+def test_experts_forward(T, D, F, E, k, drop, form):
     x, w, ids, ws, res, _ = _inputs(T, D, F, E, k, drop)
     ref = experts_ref(x, w, ids, *ws, residual=res)
     out = ops.moe_experts(x, w, ids, *ws, residual=res)
@@ -154,7 +162,7 @@ def test_experts_forward(T, D, F, E, k, drop):
 
 @pytest.mark.parametrize("w_dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("T,D,F,E,k,drop", SIZES)
-def test_experts_gradients(T, D, F, E, k, drop, w_dtype):
+def test_experts_gradients(T, D, F, E, k, drop, w_dtype, form):
     x, w, ids, ws, res, dout = _inputs(T, D, F, E, k, drop)
     leaves = [t.detach().requires_grad_() for t in (x, w.to(w_dtype), *ws, res)]
     out = ops.moe_experts(leaves[0], leaves[1], ids, *leaves[2:5], residual=leaves[5])
@@ -169,7 +177,7 @@ def test_experts_gradients(T, D, F, E, k, drop, w_dtype):
 
 
 @pytest.mark.parametrize("T,E,k", [(900, 64, 2), (900, 4, 4), (3, 16, 5), (4, 8, 4), (40, 300, 8)])
-def test_experts_all_tokens_at_one_expert_or_spread_thin(T, E, k):
+def test_experts_all_tokens_at_one_expert_or_spread_thin(T, E, k, form):
     x, w, ids, ws, res, dout = _inputs(T, 64, 72, E, k, 0.0)
     ids[:] = E - 1  # the same expert in every slot of every token
     leaves = [t.detach().requires_grad_() for t in (x, w, *ws)]

@@ -77,9 +77,10 @@ def test_plan_matches_a_loop(tokens, k, experts):
     counts, offsets, slots, rows = plan_ref(ids, experts)
     assert p.counts.tolist() == counts and p.offsets.tolist() == offsets
     assert p.slots.shape == ids.shape and p.slots.reshape(-1).tolist() == slots and p.rows.tolist() == rows
-    tiles = p.tiles[1:1 + int(p.tiles[0, 0])].tolist()
-    assert [(e, r) for e in range(experts) for r in range(offsets[e], offsets[e + 1], 128)] == [(t[0], t[1]) for t in tiles]
-    assert all(t[2] == offsets[t[0] + 1] for t in tiles)
+    for got, size in ((p.tiles, 128), (p.pairs, 256)):
+        tiles = got[1:1 + int(got[0, 0])].tolist()
+        assert [(e, r) for e in range(experts) for r in range(offsets[e], offsets[e + 1], size)] == [(t[0], t[1]) for t in tiles]
+        assert all(t[2] == offsets[t[0] + 1] for t in tiles)
 
 
 def test_plan_refuses():
