@@ -252,21 +252,30 @@ def moe_plan(experts: Tensor, n_experts: int) -> MoEPlan:
     n, E = experts.numel(), int(n_experts)
     if not experts.is_cuda or n == 0:
         return _plan_torch(experts, E)
-    ids = experts.contiguous()
-    R, blocks = rows_bound(n, E), -(-n // PLAN_CHUNK)
-    # tiles come first: they are read as 16-byte entries
-    sizes = [4 * (1 + _tiles_bound(n, E)), 4 * (1 + _tiles_bound(n, E, 2 * TILE_ROWS)), E, E + 1, n, R]
-    if blocks > 1:
-        sizes.append(blocks * E)
-    tiles, pairs, counts, offsets, slots, rows, *hist = torch.empty(sum(sizes), dtype=torch.int32, device=ids.device).split_with_sizes(sizes)
-    at = tiles.data_ptr()
-    o = [at]
-    for z in sizes:
-        o.append(o[-1] + 4 * z)
-    _call(ids, "kb_moe_plan", ids.data_ptr(), ids.dtype == torch.int64, n, E, R, o[2], o[3], o[4], o[5], at, o[1], o[6] if hist else None)
-    if hist:
-        _lib.add_launches(1)
+    buf, sizes = _plan_buffer(experts.contiguous(), n, E)
+    tiles, pairs, counts, offsets, slots, rows, *_ = buf.split_with_sizes(sizes)
     return MoEPlan(counts, offsets, slots.view(experts.shape), rows, tiles.view(-1, 4), pairs.view(-1, 4))
+
+
+def _plan_buffer(ids: Tensor, n: int, E: int) -> Tuple[Tensor, list]:
+    """The plan as one int32 buffer: (tiles, pairs, counts, offsets, slots, rows, scratch), of these sizes.  The tiles come
+    first: they are read as 16-byte entries."""
+    R, blocks = rows_bound(n, E), -(-n // PLAN_CHUNK)
+    sizes = [4 * (1 + _tiles_bound(n, E)), 4 * (1 + _tiles_bound(n, E, 2 * TILE_ROWS)), E, E + 1, n, R, blocks * E if blocks > 1 else 0]
+    buf = torch.empty(sum(sizes), dtype=torch.int32, device=ids.device)
+    tiles, pairs, counts, offsets, slots, rows, hist = _addresses(buf, sizes)
+    _call(ids, "kb_moe_plan", ids.data_ptr(), ids.dtype == torch.int64, n, E, R, counts, offsets, slots, rows, tiles, pairs, hist)
+    if blocks > 1:
+        _lib.add_launches(1)
+    return buf, sizes
+
+
+def _addresses(buf: Tensor, sizes) -> list:
+    at, out = buf.data_ptr(), []
+    for n in sizes:
+        out.append(at)
+        at += 4 * n
+    return out
 
 
 # ---------------------------------------------------------------------------------------
@@ -347,10 +356,20 @@ class _Space:
         return self.buf.data_ptr() + self.offset[name] if name in self.offset else None
 
 
-def _experts_forward(x, weights, residual, plan, groups, train):
+def _plan_at(tensors, sizes, pair):
+    """Addresses of (offsets, slots, rows, tiles) in a plan's buffer (with its sizes) or in the tensors of a MoEPlan."""
+    if sizes is None:
+        _, offsets, slots, rows, tiles, pairs = (t.data_ptr() for t in tensors)
+    else:
+        tiles, pairs, _, offsets, slots, rows, _ = _addresses(tensors[0], sizes)
+    return offsets, slots, rows, pairs if pair else tiles
+
+
+def _experts_forward(x, weights, residual, plan, sizes, groups, train):
     """(out, scratch, stacked weights); with ``train`` the scratch keeps what the backward pass reads."""
     wg, wu, wd = (_stacked(g) for g in groups)
-    (T, D), k, E, F, R = x.shape, weights.shape[1], wg.shape[0], wg.shape[1], plan.rows.numel()
+    (T, D), k, E, F = x.shape, weights.shape[1], wg.shape[0], wg.shape[1]
+    R = rows_bound(T * k, E)
     wide, hidden = 2 * R * D, 2 * R * F
     pair = _use_pairs(T * k, E)
     if train:
@@ -361,8 +380,8 @@ def _experts_forward(x, weights, residual, plan, groups, train):
         sp = _Space(x.device, xs=wide, rw=4 * R, h=hidden)
         y = sp["xs"]
     out = torch.empty((T, D), dtype=x.dtype, device=x.device)
-    _call(x, "kb_moe_experts_fwd", x.data_ptr(), x.stride(0), weights.data_ptr(), weights.dtype == torch.float32, plan.offsets.data_ptr(),
-          plan.slots.data_ptr(), plan.rows.data_ptr(), (plan.pairs if pair else plan.tiles).data_ptr(), pair, *_where(wg), *_where(wu), *_where(wd), _p(residual),
+    _call(x, "kb_moe_experts_fwd", x.data_ptr(), x.stride(0), weights.data_ptr(), weights.dtype == torch.float32, *_plan_at(plan, sizes, pair), pair,
+          *_where(wg), *_where(wu), *_where(wd), _p(residual),
           0 if residual is None else residual.stride(0), out.data_ptr(), sp["xs"], sp["rw"], sp["g"], sp["u"], sp["h"], y, T, k, D, F, E, R)
     _lib.add_launches(3)
     return out, sp, (wg, wu, wd)
@@ -370,38 +389,39 @@ def _experts_forward(x, weights, residual, plan, groups, train):
 
 class _ExpertsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weights, residual, plan, n_each, *ws):
+    def forward(ctx, x, weights, residual, plan, sizes, n_each, *ws):
         groups = [ws[i * n_each:(i + 1) * n_each] for i in range(3)]
-        out, sp, stacks = _experts_forward(x, weights, residual, plan, groups, True)
-        ctx.save_for_backward(sp.buf, *stacks, plan.offsets, plan.slots, plan.rows, plan.tiles, plan.pairs)
-        ctx.space, ctx.groups, ctx.n_each, ctx.w_dtype = sp.offset, groups, n_each, weights.dtype
+        out, sp, stacks = _experts_forward(x, weights, residual, plan, sizes, groups, True)
+        ctx.save_for_backward(sp.buf, *stacks, *plan)
+        ctx.space, ctx.sizes, ctx.groups, ctx.n_each, ctx.routing = sp.offset, sizes, groups, n_each, (weights.shape, weights.dtype)
         for i, w in enumerate(ws):
-            if ctx.needs_input_grad[5 + i]:
+            if ctx.needs_input_grad[6 + i]:
                 _count_use(w)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        buf, wg, wu, wd, offsets, slots, rows, tiles, pairs = ctx.saved_tensors
-        (T, k), (E, F, D), R, n_each, need = slots.view(-1, slots.shape[-1]).shape, wg.shape, rows.numel(), ctx.n_each, ctx.needs_input_grad
+        buf, wg, wu, wd, *plan = ctx.saved_tensors
+        ((T, k), w_dtype), (E, F, D), n_each, need = ctx.routing, wg.shape, ctx.n_each, ctx.needs_input_grad
+        R = rows_bound(T * k, E)
         at = {name: buf.data_ptr() + o for name, o in ctx.space.items()}
         pair = _use_pairs(T * k, E)
         dout = _rows2d(dout)
         dev = dout.device
         sp = _Space(dev, dys=2 * R * D, dg=2 * R * F, du=2 * R * F, part=4 * R * -(-F // 256))
         dx = torch.empty((T, D), dtype=dout.dtype, device=dev) if need[0] else None
-        dw = torch.empty((T, k), dtype=ctx.w_dtype, device=dev) if need[1] else None
-        mains = [_grad_view(g) for g in ctx.groups] if all(need[5:]) else [None]
+        dw = torch.empty((T, k), dtype=w_dtype, device=dev) if need[1] else None
+        mains = [_grad_view(g) for g in ctx.groups] if all(need[6:]) else [None]
         into = all(m is not None for m in mains)
         if into:    # accumulate straight into the flat gradient buffer
             grads = mains
         else:
-            gate_up, down = any(need[5:5 + 2 * n_each]), any(need[5 + 2 * n_each:])
+            gate_up, down = any(need[6:6 + 2 * n_each]), any(need[6 + 2 * n_each:])
             grads = [torch.empty(w.shape, dtype=w.dtype, device=dev) if wanted else None for w, wanted in ((wg, gate_up), (wu, gate_up), (wd, down))]
         where = [v for g in grads for v in (_where(g) if g is not None else (None, 0, 0))]
-        _call(dout, "kb_moe_experts_bwd", dout.data_ptr(), dout.stride(0), at["xs"], at["rw"], at["g"], at["u"], at["h"], offsets.data_ptr(),
-              slots.data_ptr(), rows.data_ptr(), (pairs if pair else tiles).data_ptr(), pair, *_where(wg), *_where(wu), *_where(wd), sp["dys"], sp["dg"], sp["du"], sp["part"],
-              _p(dx), _p(dw), ctx.w_dtype == torch.float32, *where, into, T, k, D, F, E, R)
+        _call(dout, "kb_moe_experts_bwd", dout.data_ptr(), dout.stride(0), at["xs"], at["rw"], at["g"], at["u"], at["h"],
+              *_plan_at(plan, ctx.sizes, pair), pair, *_where(wg), *_where(wu), *_where(wd), sp["dys"], sp["dg"], sp["du"], sp["part"],
+              _p(dx), _p(dw), w_dtype == torch.float32, *where, into, T, k, D, F, E, R)
         _lib.add_launches(1 + (grads[2] is not None) + (dx is not None) + (dx is not None or dw is not None) + (grads[0] is not None))
         out = []
         for i, group in enumerate(ctx.groups):
@@ -411,9 +431,9 @@ class _ExpertsFn(torch.autograd.Function):
                     _use_done(w)
                 out += [None] * n_each
             else:
-                wanted = need[5 + i * n_each:5 + (i + 1) * n_each]
+                wanted = need[6 + i * n_each:6 + (i + 1) * n_each]
                 out += [(grads[i] if group[0].dim() == 3 else grads[i][j]) if wanted[j] else None for j in range(n_each)]
-        return (dx, dw, dout if need[2] else None, None, None, *out)
+        return (dx, dw, dout if need[2] else None, None, None, None, *out)
 
 
 def _experts_small(x, w, ids, res, wg, wu, wd) -> Tensor:
@@ -480,7 +500,8 @@ def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up
     every = groups[0] + groups[1] + groups[2] + ((weights, x) if residual is None else (weights, x, residual))
     if experts.device != x.device or any(t.device != x.device for t in every):
         raise ValueError("moe_experts: all tensors must be on one device")
-    if plan is not None and (plan.slots.shape != ids_shape or plan.counts.numel() != E or plan.rows.device != x.device):
+    if plan is not None and (plan.slots.shape != ids_shape or plan.counts.numel() != E or plan.rows.device != x.device
+                             or plan.rows.numel() != rows_bound(experts.numel(), E)):
         raise ValueError("moe_experts: the plan is not one of these experts")
     k = ids_shape[-1]
     if len(shape) != 2:
@@ -495,9 +516,12 @@ def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up
     if not train and experts.numel() <= SMALL:
         out = _experts_small(x, weights, experts.contiguous(), residual, *(_stacked(g) for g in groups))
     else:
-        plan = moe_plan(experts, E) if plan is None else plan
+        sizes = None
+        if plan is None:
+            buf, sizes = _plan_buffer(experts.contiguous(), experts.numel(), E)
+            plan = (buf,)
         if train:
-            out = _ExpertsFn.apply(x, weights, residual, plan, len(groups[0]), *(w for g in groups for w in g))
+            out = _ExpertsFn.apply(x, weights, residual, plan, sizes, len(groups[0]), *groups[0], *groups[1], *groups[2])
         else:
-            out = _experts_forward(x, weights, residual, plan, groups, False)[0]
+            out = _experts_forward(x, weights, residual, plan, sizes, groups, False)[0]
     return out if len(shape) == 2 else out.view(shape)
