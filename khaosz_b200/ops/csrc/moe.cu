@@ -78,32 +78,57 @@ struct RouteParams {
 // a step for adding the bias.  Two scores further apart than this are in the right order.
 __device__ __forceinline__ float near_score(float c) { return 2e-6f + fabsf(c) * 2.4e-7f; }
 
-// The groups that may be chosen from, as bits; `close`: the last one taken and the first one left are nearer
-// than `slack` times the error of a score.  WIDE keys are exact.
+// A group's score from its lanes' two largest keys.
+template <typename Key>
+__device__ __forceinline__ Key group_score(Key best, Key next, bool two, int lane) {
+  const Key top = warp_max_key(best);
+  if (!two) return top;
+  if (lane == __ffs(__ballot_sync(FULL, best == top)) - 1) best = next;  // one holder of the largest steps back
+  return key_of(value_of(top) + value_of(warp_max_key(best)));
+}
+
+// Leaves the keys of the best groups; `close`: the last group taken and the first one left are nearer than the
+// error of their scores (fp64 keys are exact).  Groups of whole registers (a multiple of 32 experts) need no
+// index arithmetic per expert.
 template <int VPL, typename Key>
-__device__ __forceinline__ unsigned best_groups(const Key (&key)[VPL], const RouteParams& p, int lane, bool& close) {
-  constexpr bool EXACT = sizeof(Key) == 8;
+__device__ __forceinline__ void only_best_groups(Key (&key)[VPL], const RouteParams& p, int lane, bool& close) {
   const int gs = p.E / p.n_groups;
   const bool two = p.group_top == 2 && gs > 1;
+  const int per = gs / 32;  // registers of a group
+  const bool aligned = per * 32 == gs;
   Key mine = 0;  // lane g: the key of group g
-  for (int g = 0; g < p.n_groups; ++g) {
-    const int lo = g * gs, hi = lo + gs;
-    Key best = 0, next = 0;  // this lane's two largest of the group
+  if (aligned) {
+    Key best = 0, next = 0;
+    int left = per, g = 0;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const int e = i * 32 + lane;
-      if (i * 32 + 31 < lo || i * 32 >= hi) continue;  // uniform
-      const Key k = e >= lo && e < hi ? key[i] : Key(0);
-      if (k > best) { next = best; best = k; }
-      else if (k > next) next = k;
+      if (g == p.n_groups) break;
+      const Key k = key[i];
+      next = k > best ? best : (k > next ? k : next);
+      best = k > best ? k : best;
+      if (--left == 0) {
+        const Key score = group_score(best, next, two, lane);
+        if (lane == g) mine = score;
+        best = next = 0;
+        left = per;
+        ++g;
+      }
     }
-    const Key top = warp_max_key(best);
-    Key score = top;
-    if (two) {  // one holder of the largest steps back
-      if (lane == __ffs(__ballot_sync(FULL, best == top)) - 1) best = next;
-      score = key_of(value_of(top) + value_of(warp_max_key(best)));
+  } else {
+    for (int g = 0; g < p.n_groups; ++g) {
+      const int lo = g * gs, hi = lo + gs;
+      Key best = 0, next = 0;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        if (i * 32 + 31 < lo || i * 32 >= hi) continue;  // uniform
+        const int e = i * 32 + lane;
+        const Key k = e >= lo && e < hi ? key[i] : Key(0);
+        next = k > best ? best : (k > next ? k : next);
+        best = k > best ? k : best;
+      }
+      const Key score = group_score(best, next, two, lane);
+      if (lane == g) mine = score;
     }
-    if (lane == g) mine = score;
   }
   unsigned keep = 0;
   Key last = 0;
@@ -113,53 +138,86 @@ __device__ __forceinline__ unsigned best_groups(const Key (&key)[VPL], const Rou
     keep |= 1u << g;
     if (lane == g) mine = 0;
   }
-  if (!EXACT && p.topk_groups < p.n_groups) {
+  if (sizeof(Key) == 4 && p.topk_groups < p.n_groups) {
     const float a = (float)value_of(last), b = (float)value_of(warp_max_key(mine));
     close |= !(a - b > 2.f * near_score(a));
   }
-  return keep;
+  if (aligned) {
+    int left = per;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      if (!(keep & 1u)) key[i] = 0;
+      if (--left == 0) {
+        keep >>= 1;
+        left = per;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = i * 32 + lane;
+      if (e >= p.E || !(keep >> (e / gs) & 1u)) key[i] = 0;
+    }
+  }
 }
 
-// Lane j < k ends with the j-th expert in descending order of the keys.  `close` as above, for neighbours.
-template <int VPL, typename Key, typename T, bool TOLD>
-__device__ __forceinline__ int take_best(Key (&key)[VPL], const RouteParams& p, const T* zrow, int lane, bool& close) {
-  int mine = 0, prev_e = 0;
-  float prev = 0.f;
-  const int rounds = TOLD && p.k < p.E ? p.k + 1 : p.k;  // the first one left behind counts too
-  for (int j = 0; j < rounds; ++j) {
-    Key best = 0;
+// Lane j < k ends with the j-th expert in descending order of the keys, exactly.
+template <int VPL, typename Key>
+__device__ __forceinline__ int take_best(Key (&key)[VPL], const RouteParams& p, int lane) {
+  int mine = 0;
+  for (int j = 0; j < p.k; ++j) {
+    Key best = key[0];
+    int at = lane;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) best = key[i] > best ? key[i] : best;
-    const Key top = warp_max_key(best);
-    if (TOLD && top == 0) break;  // nothing is left to be chosen
-    int at = p.E;
-#pragma unroll
-    for (int i = VPL - 1; i >= 0; --i)
-      if (key[i] == top) at = i * 32 + lane;
-    const int e = (int)__reduce_min_sync(FULL, (unsigned)at);
-#pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (e == i * 32 + lane) key[i] = 0;
-    if (lane == j) mine = e;
-    if constexpr (TOLD) {
-      const float c = (float)value_of(top);
-      if (j && !(prev - c > near_score(prev)) && c != -INFINITY)
-        close |= !(to_f(zrow[e]) == to_f(zrow[prev_e]) && (!p.bias || p.bias[e] == p.bias[prev_e]));
-      prev = c;
-      prev_e = e;
+    for (int i = 1; i < VPL; ++i) {
+      at = key[i] > best ? i * 32 + lane : at;
+      best = key[i] > best ? key[i] : best;
     }
+    const Key top = warp_max_key(best);
+    const int e = (int)__reduce_min_sync(FULL, best == top ? (unsigned)at : ~0u);
+    if (e == at) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (at == i * 32 + lane) key[i] = 0;
+    }
+    if (lane == j) mine = e;
   }
   return mine;
 }
 
-template <int VPL, typename Key>
-__device__ __forceinline__ void only_groups(Key (&key)[VPL], const RouteParams& p, int lane, unsigned keep) {
-  const int gs = p.E / p.n_groups;
+// The same for fp32 scores.  The low five bits of a key give way to the register's number, which makes a lane's
+// keys unique and the lowest index the largest of equals (the ALU pipe bounds this kernel: fewer compares); the
+// lost bits count as error.  `close`: two neighbours in the ranking, the first expert left behind among them, are
+// within their errors of one another and do not come from the same logit and bias.
+constexpr unsigned NUMBER = 31u;
+__device__ __forceinline__ float near_key(float c) { return near_score(c) + fabsf(c) * 7.7e-6f; }  // 2^-17 and a bit
+template <int VPL, typename T>
+__device__ __forceinline__ int take_best_scored(uint32_t (&key)[VPL], const RouteParams& p, const T* zrow, int lane, bool& close) {
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    const int e = i * 32 + lane;
-    if (e >= p.E || !(keep >> (e / gs) & 1u)) key[i] = 0;
+  for (int i = 0; i < VPL; ++i) key[i] = key[i] ? (key[i] & ~NUMBER) | (NUMBER - i) : 0u;
+  int mine = 0, prev_e = 0;
+  float prev = 0.f;
+  const int rounds = p.k < p.E ? p.k + 1 : p.k;
+  for (int j = 0; j < rounds; ++j) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int i = 1; i + 1 < VPL; i += 2) best = __vimax3_u32(best, key[i], key[i + 1]);
+    if (VPL % 2 == 0) best = max(best, key[VPL - 1]);
+    const uint32_t top = __reduce_max_sync(FULL, best);
+    if (top == 0) break;  // nothing is left to be chosen
+    const int who = __ffs(__ballot_sync(FULL, best == top)) - 1;
+    const uint32_t gone = lane == who ? top : 1u;  // no key is 1
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) key[i] = key[i] == gone ? 0u : key[i];
+    const int e = (int)(NUMBER - (top & NUMBER)) * 32 + who;
+    if (lane == j) mine = e;
+    const float c = value_of(top & ~NUMBER);
+    if (j && !(prev - c > near_key(prev)) && c > -3e38f)
+      close |= !(to_f(zrow[e]) == to_f(zrow[prev_e]) && (!p.bias || p.bias[e] == p.bias[prev_e]));
+    prev = c;
+    prev_e = e;
   }
+  return mine;
 }
 
 // The whole ranking in fp64.
@@ -187,8 +245,8 @@ __device__ __noinline__ int rank_wide(const RouteParams& p, const T* zrow, int l
     }
   }
   bool close = false;
-  if (p.n_groups > 1) only_groups(key, p, lane, best_groups(key, p, lane, close));
-  return take_best<VPL, uint64_t, T, false>(key, p, zrow, lane, close);
+  if (p.n_groups > 1) only_best_groups(key, p, lane, close);
+  return take_best(key, p, lane);
 }
 
 // The selected experts' weights from their own logits; lane j < k holds slot j.  With renormalisation the
@@ -260,9 +318,9 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(const RouteParams p) {
     for (int i = 0; i < VPL; ++i) key[i] = i * 32 + lane < p.E ? key_of(z[i]) : 0u;
     if (p.n_groups > 1) {
       bool exact = false;  // a group counts its largest logit: nothing is rounded
-      only_groups(key, p, lane, best_groups(key, p, lane, exact));
+      only_best_groups(key, p, lane, exact);
     }
-    mine = take_best<VPL, uint32_t, T, false>(key, p, zrow, lane, close);
+    mine = take_best(key, p, lane);
   } else {
     const float inv = row_sum > 0.f ? 1.f / row_sum : 0.f;
 #pragma unroll
@@ -272,15 +330,14 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(const RouteParams p) {
       key[i] = i * 32 + lane < p.E ? key_of(c) : 0u;
     }
     if (p.n_groups > 1) {
-      const unsigned keep = best_groups(key, p, lane, close);
+      only_best_groups(key, p, lane, close);
       if (!p.bias) {  // inside the groups the logits tell the order
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
           if (key[i]) key[i] = key_of(z[i]);
       }
-      only_groups(key, p, lane, keep);
     }
-    mine = p.bias ? take_best<VPL, uint32_t, T, true>(key, p, zrow, lane, close) : take_best<VPL, uint32_t, T, false>(key, p, zrow, lane, close);
+    mine = p.bias ? take_best_scored(key, p, zrow, lane, close) : take_best(key, p, lane);
     if (close) mine = rank_wide<VPL, T>(p, zrow, lane, m);  // uniform in the warp
   }
   const bool slot = lane < p.k;
