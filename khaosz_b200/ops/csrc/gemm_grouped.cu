@@ -36,14 +36,16 @@ constexpr int BK = 64;
 constexpr int UMMA_K = 16;
 constexpr int A_BYTES = BM * BK * 2;
 constexpr int ATOM_BYTES = BK * 128;
-constexpr int EPI_WARPS = 4;  // one per TMEM lane quarter (eight measured slower: GATE_UP 347 against 329 us)
-constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
-constexpr int STAGING = 32 * 128;  // DHID: bytes of one warp's 32 rows x 64 bf16, for each of its two operands
+constexpr int STAGING = 32 * 64;  // DHID: bytes of one warp's 32 rows x 32 bf16, for each of its two operands
 template <int MODE, bool PAIR>
 struct Cfg {
+  // epilogue warps: one per TMEM lane quarter; DHID, whose epilogue is the longest, has two, each with half of the columns
+  // (200 us with one; for GATE_UP two measured slower, 347 against 329 us)
+  static constexpr int EPI = MODE == DHID ? 8 : 4;
+  static constexpr int THREADS = 64 + 32 * EPI;
   static constexpr int B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2;
   static constexpr int STAGES = PAIR ? (MODE == DHID ? 6 : 7) : 4;
-  static constexpr int STAGING_BYTES = MODE == DHID ? EPI_WARPS * 2 * STAGING : 0;
+  static constexpr int STAGING_BYTES = MODE == DHID ? EPI * 2 * STAGING : 0;
   static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + STAGING_BYTES + 256 + 1024;
 };
 static_assert(BM == 128 && KB_MOE_ROW_ALIGN == UMMA_K, "a segment begins on a K step");
@@ -51,6 +53,7 @@ static_assert(BM == 128 && KB_MOE_ROW_ALIGN == UMMA_K, "a segment begins on a K 
 struct Params {
   const int4* tiles;    // row modes: [0].x tiles, then (expert, first row, end row, 0)
   const int* offsets;   // weight-gradient modes: [E + 1]
+  const int* order;     // weight-gradient modes: [E] the experts by falling number of rows
   int E, num_m, num_n;  // weight-gradient modes: M tiles of one matrix; all: N tiles
   int num_k;            // row modes: K blocks (DX: of one of the two halves)
   int M, N;             // valid rows of a weight gradient; valid columns
@@ -58,7 +61,7 @@ struct Params {
   long ld0, ld1, stride0, stride1;  // pitch and (weight gradients) distance of the experts
   const __nv_bfloat16 *g, *u;       // DHID: [rows, N]
   const float* rw;                  // GATE_UP, DHID: routing weight of a row
-  float* part;                      // DHID: [rows, num_n]
+  float* part;                      // DHID: [rows, 2 num_n]
   int accumulate;                   // weight gradients: add to what is there
   int* err;
 };
@@ -99,8 +102,9 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int u, int total, int r
   } else {
     // the 128-row blocks of an expert's matrix, or of its two matrices one after the other; a pair takes two of them
     const int blocks = MODE == DW_GU ? 2 * p.num_m : p.num_m, units = PAIR ? (blocks + 1) / 2 : blocks;
-    r.e = x / units;
-    const int m = (x - r.e * units) * (PAIR ? 2 : 1) + (PAIR ? rank : 0);
+    const int place = x / units;
+    r.e = __ldg(p.order + place);
+    const int m = (x - place * units) * (PAIR ? 2 : 1) + (PAIR ? rank : 0);
     r.mat = MODE == DW_GU && m >= p.num_m;
     r.m0 = (m - (r.mat ? p.num_m : 0)) * BM;
     r.k0 = __ldg(p.offsets + r.e);
@@ -201,10 +205,12 @@ __device__ __forceinline__ void unpack8(const uint4& v, float* f) {
   const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
   f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
 }
+// Piece `piece` (16 bytes) of a staging row of 64 bytes: eight rows' same piece lie in eight different bank groups.
+__device__ __forceinline__ uint32_t staged(uint32_t row, uint32_t piece) { return row * 64u + ((piece ^ (row >> 1 & 3u)) << 4); }
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
 template <int MODE, bool PAIR>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(Cfg<MODE, PAIR>::THREADS, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a2,
                const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_b2, const Params p) {
   constexpr bool A_MN = MODE >= DW_DOWN;
@@ -228,6 +234,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   const int lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_rank() : 0;
   const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  // the i-th unit of this CTA (or pair): every other round runs backwards, so that units of falling length even out
+  auto nth = [&](int i) { return i * step + (i & 1 ? step - 1 - first : first); };
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < STAGES; ++i) {
@@ -236,7 +244,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], (PAIR ? 2 : 1) * EPI_WARPS);
+      mbar_init(&tempty[i], (PAIR ? 2 : 1) * C::EPI);
     }
     mbar_fence_init();
     tma_prefetch_desc(&tmap_a);
@@ -266,7 +274,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int un = first; un < total && ok; un += step) {
+      for (int it = 0, un = nth(0); it * step < total && ok; un = nth(++it)) {
+        if (un >= total) continue;
         const Unit t = unit_of<MODE, PAIR>(p, un, total, rank);
         const int nk = k_blocks<MODE>(p, t);
         const int cols = tile_cols<MODE, PAIR>(p, t);
@@ -330,7 +339,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       int acc = 0;
       uint32_t aph = 0;
       bool ok = true;
-      for (int un = first; un < total && ok; un += step) {
+      for (int it = 0, un = nth(0); it * step < total && ok; un = nth(++it)) {
+        if (un >= total) continue;
         Unit t{};
         if constexpr (MODE >= DW_DOWN) t = unit_of<MODE, PAIR>(p, un, total, 0);
         else column_of<MODE, PAIR>(p, un, total, t.row0, t.n0);
@@ -380,26 +390,29 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     const int row = q * 32 + lane;
     int acc = 0;
     uint32_t aph = 0;
-    for (int un = first; un < total; un += step) {
+    for (int it = 0, un = nth(0); it * step < total; un = nth(++it)) {
+      if (un >= total) continue;
       const Unit t = unit_of<MODE, PAIR>(p, un, total, rank);
       const bool any_k = k_blocks<MODE>(p, t) > 0;
       float w = 0.f;
       if constexpr (MODE == GATE_UP || MODE == DHID)
         if (t.row0 + row < t.end) w = p.rw[t.row0 + row];
-      // DHID: G and U come and dG and dU go in whole lines, eight lanes to a row's 64 columns, through the warp's own
-      // staging rows (16-byte pieces swizzled by the row); a lane that walked its own row would touch 32 lines per
-      // access, which held the tensor cores up (the kernel took 241 us so, now 215, of a main loop of 150).
+      // DHID: G and U come and dG and dU go through the warp's own staging rows, four lanes to a row's 32 columns (16-byte
+      // pieces swizzled by the row); a lane that walked its own row would touch 32 lines per access, which held the
+      // tensor cores up (the kernel took 241 us so).  The first columns are under way before the accumulator is.
+      constexpr int CHUNKS = BN / 32 / (C::EPI / 4);
+      const int chunk0 = ((warp - 2) >> 2) * CHUNKS;
       uint8_t* sg = staging + (warp - 2) * 2 * STAGING;
       uint8_t* su = sg + STAGING;
-      const int r8 = lane >> 3, c8 = lane & 7;
+      const int r4 = lane >> 2, c4 = lane & 3;
       const size_t row0 = t.row0 + q * 32;
       const int rows = min(32, t.end - (t.row0 + q * 32));
-      uint4 vg[8], vu[8];
+      uint4 vg[4], vu[4];
       auto fetch = [&](int c) {
-        const int col = t.n0 + c * 64 + c8 * 8;
+        const int col = t.n0 + c * 32 + c4 * 8;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = i * 4 + r8;
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + r4;
           vg[i] = vu[i] = make_uint4(0u, 0u, 0u, 0u);
           if (r < rows && col < p.N) {
             vg[i] = *reinterpret_cast<const uint4*>(p.g + (row0 + r) * p.ld0 + col);
@@ -407,7 +420,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           }
         }
       };
-      if constexpr (MODE == DHID) fetch(0);
+      if constexpr (MODE == DHID) fetch(chunk0);
       if (any_k && !mbar_wait(&tfull[acc], aph, abort_flag, p.err, KB_ERR_TIMEOUT_TMEM_FULL)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
@@ -445,52 +458,49 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           } else if constexpr (MODE == DHID) {
             float dot = 0.f;
 #pragma unroll 1
-            for (int c = 0; c < BN / 64; ++c) {
-              if (t.n0 + c * 64 >= p.N) break;
+            for (int c = chunk0; c < chunk0 + CHUNKS; ++c) {
+              if (t.n0 + c * 32 >= p.N) break;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + r8;
-                *reinterpret_cast<uint4*>(sg + sw128_offset(r, c8)) = vg[i];
-                *reinterpret_cast<uint4*>(su + sw128_offset(r, c8)) = vu[i];
+              for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + r4;
+                *reinterpret_cast<uint4*>(sg + staged(r, c4)) = vg[i];
+                *reinterpret_cast<uint4*>(su + staged(r, c4)) = vu[i];
               }
               __syncwarp();
-              if (c + 1 < BN / 64 && t.n0 + (c + 1) * 64 < p.N) fetch(c + 1);  // under way during the arithmetic
+              if (c + 1 < chunk0 + CHUNKS && t.n0 + (c + 1) * 32 < p.N) fetch(c + 1);  // under way during the arithmetic
+              uint32_t v[32];
+              tmem_ld_32x32b_x32(t_row + c * 32, v);
+              tmem_ld_wait();
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(t_row + c * 64 + h * 32, v);
-                tmem_ld_wait();
+              for (int i = 0; i < 4; ++i) {
+                uint4* pg = reinterpret_cast<uint4*>(sg + staged(lane, i));
+                uint4* pu = reinterpret_cast<uint4*>(su + staged(lane, i));
+                float g[8], u[8], dg[8], du[8];
+                unpack8(*pg, g);
+                unpack8(*pu, u);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  uint4* pg = reinterpret_cast<uint4*>(sg + sw128_offset(lane, h * 4 + i));
-                  uint4* pu = reinterpret_cast<uint4*>(su + sw128_offset(lane, h * 4 + i));
-                  float g[8], u[8], dg[8], du[8];
-                  unpack8(*pg, g);
-                  unpack8(*pu, u);
-#pragma unroll
-                  for (int x = 0; x < 8; ++x) {
-                    const float d = __uint_as_float(v[i * 8 + x]), s = sigmoid(g[x]), act = g[x] * s;
-                    dot += d * (act * u[x]);
-                    dg[x] = w * d * u[x] * (s + act * (1.f - s));
-                    du[x] = w * d * act;
-                  }
-                  *pg = pack8(dg);
-                  *pu = pack8(du);
+                for (int x = 0; x < 8; ++x) {
+                  const float d = __uint_as_float(v[i * 8 + x]), s = sigmoid(g[x]), act = g[x] * s, da = d * act;
+                  dot = fmaf(da, u[x], dot);
+                  dg[x] = w * (d * u[x]) * fmaf(act, 1.f - s, s);
+                  du[x] = w * da;
                 }
+                *pg = pack8(dg);
+                *pu = pack8(du);
               }
               __syncwarp();
-              const int col = t.n0 + c * 64 + c8 * 8;
+              const int col = t.n0 + c * 32 + c4 * 8;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + r8;
+              for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + r4;
                 if (r < rows && col < p.N) {
-                  *reinterpret_cast<uint4*>(p.out0 + (row0 + r) * p.ld0 + col) = *reinterpret_cast<const uint4*>(sg + sw128_offset(r, c8));
-                  *reinterpret_cast<uint4*>(p.out1 + (row0 + r) * p.ld0 + col) = *reinterpret_cast<const uint4*>(su + sw128_offset(r, c8));
+                  *reinterpret_cast<uint4*>(p.out0 + (row0 + r) * p.ld0 + col) = *reinterpret_cast<const uint4*>(sg + staged(r, c4));
+                  *reinterpret_cast<uint4*>(p.out1 + (row0 + r) * p.ld0 + col) = *reinterpret_cast<const uint4*>(su + staged(r, c4));
                 }
               }
               __syncwarp();
             }
-            if (live) p.part[grow * p.num_n + t.n0 / BN] = dot;
+            if (live) p.part[(grow * p.num_n + t.n0 / BN) * (C::EPI / 4) + ((warp - 2) >> 2)] = dot;
           } else {
 #pragma unroll 1
             for (int c = 0; c < BN / 32; ++c) {
@@ -589,8 +599,8 @@ static int launch_form(const CUtensorMap& a, const CUtensorMap& a2, const CUtens
       return KB_STATUS_CUDA_ERROR;
     set[dev & 63] = true;
   }
-  const cudaError_t e = PAIR ? kb::moe::launch_after<2>(grouped_kernel<MODE, PAIR>, sms / 2 * 2, NUM_THREADS, Cfg<MODE, PAIR>::SMEM, st, a, a2, b, b2, p)
-                             : kb::moe::launch_after(grouped_kernel<MODE, PAIR>, sms, NUM_THREADS, Cfg<MODE, PAIR>::SMEM, st, a, a2, b, b2, p);
+  const cudaError_t e = PAIR ? kb::moe::launch_after<2>(grouped_kernel<MODE, PAIR>, sms / 2 * 2, Cfg<MODE, PAIR>::THREADS, Cfg<MODE, PAIR>::SMEM, st, a, a2, b, b2, p)
+                             : kb::moe::launch_after(grouped_kernel<MODE, PAIR>, sms, Cfg<MODE, PAIR>::THREADS, Cfg<MODE, PAIR>::SMEM, st, a, a2, b, b2, p);
   return e == cudaSuccess ? KB_STATUS_OK : KB_STATUS_CUDA_ERROR;
 }
 template <int MODE>
@@ -647,7 +657,7 @@ extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, 
   Device d;
   KB_TRY(device(&d));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  KB_TRY(kb::moe::launch_gather(x, ldx, rows, offsets + E, weights, w_f32, rw, xs, k, D, R, d.sms, st));
+  KB_TRY(kb::moe::launch_gather(x, ldx, rows, offsets, E, nullptr, weights, w_f32, rw, xs, k, D, R, d.sms, st));
   CUtensorMap a, b, b2;
   Params p{};
   p.tiles = reinterpret_cast<const int4*>(tiles);
@@ -680,7 +690,7 @@ extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, 
 
 extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, const float* rw, const void* g, const void* u, const void* h,
                                   const int* offsets, const int* slots, const int* rows, const int* tiles, int pair, const void* wg, long ldg, long sg,
-                                  const void* wu, long ldu, long su, const void* wd, long ldd, long sd, void* dys, void* dg, void* du, float* part,
+                                  const void* wu, long ldu, long su, const void* wd, long ldd, long sd, void* dys, void* dg, void* du, float* part, int* order,
                                   void* dx, void* dw, int w_f32, void* dwg, long ldwg, long sdwg, void* dwu, long ldwu, long sdwu, void* dwd, long ldwd,
                                   long sdwd, int accumulate, int T, int k, int D, int F, int E, int R, void* stream) {
   using namespace kb::grouped;
@@ -694,18 +704,19 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
   Device d;
   KB_TRY(device(&d));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  KB_TRY(kb::moe::launch_gather(dout, ldo, rows, offsets + E, nullptr, 0, nullptr, dys, k, D, R, d.sms, st));
+  KB_TRY(kb::moe::launch_gather(dout, ldo, rows, offsets, E, order, nullptr, 0, nullptr, dys, k, D, R, d.sms, st));
   CUtensorMap a, a2, b, b2;
   Params p{};
   p.tiles = reinterpret_cast<const int4*>(tiles);
   p.offsets = offsets;
+  p.order = order;
   p.E = E;
   p.err = d.err;
   // dG, dU and the routing weights' partial gradients
-  const int n_part = cdiv(F, BN);
+  const int n_part = 2 * cdiv(F, BN);
   KB_TRY(rows_map(&a, dys, R, D, BM));
   KB_TRY(weight_map(&b, W, E, D, F, BK));
-  p.num_n = n_part;
+  p.num_n = cdiv(F, BN);
   p.num_k = cdiv(D, BK);
   p.N = F;
   p.out0 = static_cast<__nv_bfloat16*>(dg);

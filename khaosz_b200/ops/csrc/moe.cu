@@ -570,12 +570,23 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
 // passes around the products
 // ---------------------------------------------------------------------------------------
 // Grouped copy of token rows: dst[r] = src[rows[r] / k]; padding rows are zero.  One warp per row.
-// With `rw`: the row's routing weight too (0 for padding).
-__global__ void __launch_bounds__(256) gather_kernel(const __nv_bfloat16* src, long ld, const int* rows, const int* end, const void* w, int w_f32,
-                                                     float* rw, __nv_bfloat16* dst, int k, int D) {
+// With `rw`: the row's routing weight too (0 for padding).  With `order`: the last block ranks the experts by their rows.
+__global__ void __launch_bounds__(256) gather_kernel(const __nv_bfloat16* src, long ld, const int* rows, const int* offsets, int E, int* order,
+                                                     const void* w, int w_f32, float* rw, __nv_bfloat16* dst, int k, int D) {
   const int lane = threadIdx.x & 31;
   await_predecessor();
-  const int last = *end;
+  if (order && blockIdx.x == gridDim.x - 1) {
+    __shared__ int len[KB_MOE_MAX_EXPERTS];
+    for (int e = threadIdx.x; e < E; e += 256) len[e] = offsets[e + 1] - offsets[e];
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += 256) {
+      const int mine = len[e];
+      int rank = 0;
+      for (int o = 0; o < E; ++o) rank += len[o] > mine || (len[o] == mine && o < e);
+      order[rank] = e;
+    }
+  }
+  const int last = offsets[E];
   for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < last; r += gridDim.x * 8) {
     const int a = rows[r];
     uint4* o = reinterpret_cast<uint4*>(dst + (size_t)r * D);
@@ -731,10 +742,10 @@ namespace kb {
 namespace moe {
 
 // grouped copy of [T, D] rows (used by the forward and the backward pass of the products)
-int launch_gather(const void* src, long ld, const int* rows, const int* end, const void* w, int w_f32, float* rw, void* dst, int k, int D, int R, int sms,
+int launch_gather(const void* src, long ld, const int* rows, const int* offsets, int E, int* order, const void* w, int w_f32, float* rw, void* dst, int k, int D, int R, int sms,
                   cudaStream_t st) {
   const int want = (R + 7) / 8, cap = sms * 8;
-  launch_after(gather_kernel, want < cap ? want : cap, 256, 0, st, static_cast<const __nv_bfloat16*>(src), ld, rows, end, w, w_f32, rw,
+  launch_after(gather_kernel, want < cap ? want : cap, 256, 0, st, static_cast<const __nv_bfloat16*>(src), ld, rows, offsets, E, order, w, w_f32, rw,
                static_cast<__nv_bfloat16*>(dst), k, D);
   return launched();
 }

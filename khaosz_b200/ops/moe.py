@@ -408,7 +408,7 @@ class _ExpertsFn(torch.autograd.Function):
         pair = _use_pairs(T * k, E)
         dout = _rows2d(dout)
         dev = dout.device
-        sp = _Space(dev, dys=2 * R * D, dg=2 * R * F, du=2 * R * F, part=4 * R * -(-F // 256))
+        sp = _Space(dev, dys=2 * R * D, dg=2 * R * F, du=2 * R * F, part=4 * R * 2 * -(-F // 256), order=4 * E)
         dx = torch.empty((T, D), dtype=dout.dtype, device=dev) if need[0] else None
         dw = torch.empty((T, k), dtype=w_dtype, device=dev) if need[1] else None
         mains = [_grad_view(g) for g in ctx.groups] if all(need[6:]) else [None]
@@ -420,7 +420,7 @@ class _ExpertsFn(torch.autograd.Function):
             grads = [torch.empty(w.shape, dtype=w.dtype, device=dev) if wanted else None for w, wanted in ((wg, gate_up), (wu, gate_up), (wd, down))]
         where = [v for g in grads for v in (_where(g) if g is not None else (None, 0, 0))]
         _call(dout, "kb_moe_experts_bwd", dout.data_ptr(), dout.stride(0), at["xs"], at["rw"], at["g"], at["u"], at["h"],
-              *_plan_at(plan, ctx.sizes, pair), pair, *_where(wg), *_where(wu), *_where(wd), sp["dys"], sp["dg"], sp["du"], sp["part"],
+              *_plan_at(plan, ctx.sizes, pair), pair, *_where(wg), *_where(wu), *_where(wd), sp["dys"], sp["dg"], sp["du"], sp["part"], sp["order"],
               _p(dx), _p(dw), w_dtype == torch.float32, *where, into, T, k, D, F, E, R)
         _lib.add_launches(1 + (grads[2] is not None) + (dx is not None) + (dx is not None or dw is not None) + (grads[0] is not None))
         out = []
