@@ -36,7 +36,8 @@ def _time(fn, iters: int, flush: torch.Tensor):
 def main(argv=None):
     p = argparse.ArgumentParser()
     p.add_argument("kernel", choices=["gemm", "gemm_pair", "gemm_swiglu", "gemm_w8", "gemm_fp8", "flash_fwd", "flash_bwd", "rmsnorm",
-                                      "rmsnorm_bwd", "swiglu", "rope", "ce", "adamw", "decode", "sample", "embedding"])
+                                      "rmsnorm_bwd", "swiglu", "rope", "ce", "adamw", "decode", "sample", "embedding", "moe_route",
+                                      "moe_experts", "moe_experts_train"])
     p.add_argument("--m", type=int, default=4096)
     p.add_argument("--n", type=int, default=4096)
     p.add_argument("--k", type=int, default=4096)
@@ -44,6 +45,8 @@ def main(argv=None):
     p.add_argument("--seq", type=int, default=2048)
     p.add_argument("--heads", type=int, default=16)
     p.add_argument("--kv_heads", type=int, default=4)
+    p.add_argument("--experts", type=int, default=16)
+    p.add_argument("--topk", type=int, default=4)
     p.add_argument("--iters", type=int, default=5)
     a = p.parse_args(argv)
     dev = "cuda"
@@ -158,6 +161,22 @@ def main(argv=None):
         logits = torch.randn(M, 32000, device=dev, dtype=bf)
         fn = lambda: fused_sample(logits, 0.8, 50, 0.95)
         bytes_ = 2.0 * M * 32000
+    elif a.kernel == "moe_route":
+        # --m tokens; scores with a selection bias, as a balanced router uses them
+        logits, bias = torch.randn(M, a.experts, device=dev), torch.randn(a.experts, device=dev) * 0.05
+        fn = lambda: ops.moe_route(logits, a.topk, score="sigmoid", bias=bias)
+        bytes_ = 4.0 * M * a.experts + 12.0 * M * a.topk
+    elif a.kernel in ("moe_experts", "moe_experts_train"):
+        # --m tokens, --k model width, --n expert width; the training form runs forward and backward
+        train = a.kernel == "moe_experts_train"
+        x, dout = torch.randn(M, K, device=dev, dtype=bf), torch.randn(M, K, device=dev, dtype=bf)
+        weights, experts = ops.moe_route(torch.randn(M, a.experts, device=dev), a.topk)
+        ws = [torch.randn(a.experts, *shape, device=dev, dtype=bf) * 0.02 for shape in ((N, K), (N, K), (K, N))]
+        leaves = [t.requires_grad_(train) for t in (x, weights, *ws)]
+        run = lambda: ops.moe_experts(leaves[0], leaves[1], experts, *leaves[2:])
+        fn = (lambda: torch.autograd.grad(run(), leaves, dout)) if train else run
+        flops = (18.0 if train else 6.0) * M * a.topk * N * K
+        bytes_ = (2.0 if train else 1.0) * (4.0 * M * K + 6.0 * a.experts * N * K)
     else:
         table = torch.randn(32000, N, device=dev, dtype=bf)
         ids = torch.randint(0, 32000, (M,), device=dev)
