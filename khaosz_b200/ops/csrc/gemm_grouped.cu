@@ -20,7 +20,7 @@
 // Two forms.  A single CTA per tile reads (128 + 256) x 64 operands per K block: 92 bytes per clock at the tensor
 // cores' full rate, more than the about 64 that reach an SM from L2, and that bounds it (13 to 15 TB/s measured).
 // PAIR: two CTAs of a cluster compute 256 x 256 together (tcgen05 cta_group::2), each staging its own 128 rows
-// and half of B, 61 bytes per clock.  A pair's tile is wasted by experts with few rows, see use_pair().
+// and half of B, 61 bytes per clock.  Half of a pair's tile is wasted on an expert's last rows: ops/moe.py chooses.
 #include "common.cuh"
 #include "kb_api.h"
 #include "moe.cuh"

@@ -213,7 +213,7 @@ int kb_moe_route_fwd(const void* z, int z_f32, long ldz, const float* bias, void
 int kb_moe_route_bwd(const void* z, int z_f32, long ldz, const float* bias, const long long* ids, const void* dw, int w_f32, void* dz,
                      int T, int E, int k, int sigmoid, int renorm, float scale, void* stream);
 // Grouping of n assignments by expert.  counts [E], offsets [E+1], slots [n], rows [R], tiles [1 + tiles][4] (16-byte aligned,
-// R / 128 + min(E, n) tiles at most), pairs: the same of 256 rows (R / 256 + min(E, n)); R >= n + 15 min(E, n) rounded up to 16; hist [ceil(n / 2048), E] scratch (n > 2048).
+// R / 128 + min(E, n) tiles at most), pairs: the same of 256 rows (R / 256 + min(E, n)); R >= n + 15 min(E, n) rounded up to 16; hist [ceil(n / 2048) + 1, E] scratch (n > 2048).
 // An index outside 0..E-1 is dropped (slot -1).
 int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int* counts, int* offsets, int* slots, int* rows, int* tiles, int* pairs,
                 int* hist, void* stream);

@@ -74,9 +74,10 @@ struct RouteParams {
 };
 
 // What an fp32 score may be off: below 5e-7 for either kind (1/(1+e^-z): 0.25 of e's error of at most 2^-21,
-// 0.22 * 2^-22 for the rounded argument, 2^-22 for the division, 2^-24 for the sum; e/sum likewise), and half
-// a step for adding the bias.  Two scores further apart than this are in the right order.
-__device__ __forceinline__ float near_score(float c) { return 2e-6f + fabsf(c) * 2.4e-7f; }
+// 0.22 * 2^-22 for the rounded argument, 2^-22 for the division, 2^-24 for the sum; e/sum likewise, and the
+// sum of up to 32 terms per lane 1e-6 of it), and half a step for adding the bias.  Two scores further apart than
+// twice that are in the right order.
+__device__ __forceinline__ float near_score(float c) { return 3e-6f + fabsf(c) * 2.4e-7f; }
 
 // A group's score from its lanes' two largest keys.
 template <typename Key>
@@ -428,8 +429,9 @@ struct PlanParams {
   int* rows;      // [R]
   int4* tiles;    // [1 + max]: .x of the first = number of 128-row tiles, then (expert, first row, end row, 0)
   int4* pairs;    // the same of 256 rows
-  int* hist;      // [nb, E] (several blocks only)
+  int* hist;      // [nb, E], with a row for the totals where they are scanned (several blocks only)
 };
+constexpr int SCAN_FROM = 256;  // blocks from which the counts are scanned by a kernel of their own, not summed by every block
 
 __device__ __forceinline__ int expert_of(const PlanParams& p, int a) {
   if (a >= p.n) return -1;
@@ -477,6 +479,28 @@ __device__ __forceinline__ void block_prefix(int (&v)[N], int (*red)[N]) {
   for (int i = 0; i < N; ++i) v[i] = x[i] - v[i] + __reduce_add_sync(FULL, lane < warp ? red[lane][i] : 0);
 }
 
+// One block per expert: the counts of the blocks become the assignments before each block, and the total follows.
+__global__ void __launch_bounds__(PLAN_THREADS) plan_scan_kernel(const PlanParams p) {
+  __shared__ int red[32][1];
+  await_predecessor();
+  int carry = 0;
+  for (int b0 = 0; b0 < p.nb; b0 += PLAN_THREADS) {
+    const int b = b0 + threadIdx.x;
+    int* at = p.hist + (size_t)b * p.E + blockIdx.x;
+    const int mine = b < p.nb ? *at : 0;
+    int v[1] = {mine};
+    block_prefix(v, red);
+    if (b < p.nb) *at = carry + v[0];
+    // the last thread's inclusive prefix is the sum of these blocks
+    __shared__ int sum;
+    if (threadIdx.x == PLAN_THREADS - 1) sum = v[0] + mine;
+    __syncthreads();
+    carry += sum;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) p.hist[(size_t)p.nb * p.E + blockIdx.x] = carry;
+}
+
 // SINGLE: one block holds all assignments and nothing was counted before.
 template <bool SINGLE>
 __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanParams p) {
@@ -514,7 +538,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
     }
   }
   int total = SINGLE ? in_block : 0, before = 0;
-  if (!SINGLE) {  // totals over the blocks: the threads share the blocks of an expert
+  if (!SINGLE && p.nb >= SCAN_FROM) {
+    if (tid < p.E) {
+      before = p.hist[(size_t)blockIdx.x * p.E + tid];
+      total = p.hist[(size_t)p.nb * p.E + tid];
+    }
+  } else if (!SINGLE) {  // totals over the blocks: the threads share the blocks of an expert
     __shared__ int sum[1024], upto[1024];
     sum[tid] = upto[tid] = 0;
     __syncthreads();
@@ -733,6 +762,7 @@ extern "C" int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int*
     if (smem > 32 * 1024 && cudaFuncSetAttribute(plan_place_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return KB_STATUS_CUDA_ERROR;
     launch_after(plan_count_kernel, nb, PLAN_THREADS, 0, st, p);
+    if (nb >= SCAN_FROM) launch_after(plan_scan_kernel, E, PLAN_THREADS, 0, st, p);
     launch_after(plan_place_kernel<false>, nb, PLAN_THREADS, smem, st, p);
   }
   return launched();

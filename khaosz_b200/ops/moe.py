@@ -26,6 +26,7 @@ TILE_ROWS = 128     # rows of one tile of the grouped products
 MAX_EXPERTS = 1024
 MAX_SLOTS = 32      # experts per token, and groups of experts
 PLAN_CHUNK = 2048   # assignments that one block of the grouping kernel takes
+PLAN_SCAN_FROM = 256  # blocks from which their counts are scanned by a kernel of their own
 SMALL = 16          # assignments up to which a forward pass without gradients needs no grouping (see _experts_small)
 
 _KERNEL_DTYPES = (torch.bfloat16, torch.float32)
@@ -261,12 +262,12 @@ def _plan_buffer(ids: Tensor, n: int, E: int) -> Tuple[Tensor, list]:
     """The plan as one int32 buffer: (tiles, pairs, counts, offsets, slots, rows, scratch), of these sizes.  The tiles come
     first: they are read as 16-byte entries."""
     R, blocks = rows_bound(n, E), -(-n // PLAN_CHUNK)
-    sizes = [4 * (1 + _tiles_bound(n, E)), 4 * (1 + _tiles_bound(n, E, 2 * TILE_ROWS)), E, E + 1, n, R, blocks * E if blocks > 1 else 0]
+    sizes = [4 * (1 + _tiles_bound(n, E)), 4 * (1 + _tiles_bound(n, E, 2 * TILE_ROWS)), E, E + 1, n, R, (blocks + 1) * E if blocks > 1 else 0]
     buf = torch.empty(sum(sizes), dtype=torch.int32, device=ids.device)
     tiles, pairs, counts, offsets, slots, rows, hist = _addresses(buf, sizes)
     _call(ids, "kb_moe_plan", ids.data_ptr(), ids.dtype == torch.int64, n, E, R, counts, offsets, slots, rows, tiles, pairs, hist)
     if blocks > 1:
-        _lib.add_launches(1)
+        _lib.add_launches(2 if blocks >= PLAN_SCAN_FROM else 1)
     return buf, sizes
 
 

@@ -109,6 +109,25 @@ def test_plan(T, k, E, dtype):
     assert all(torch.equal(a, b) for a, b in zip(p[:4], again[:4]))
 
 
+@pytest.mark.parametrize("T,k,E", [(140000, 4, 1024), (2_500_000, 1, 7), (70000, 8, 200)])
+def test_plan_of_many_assignments(T, k, E):
+    """Against a stable sort: the loop of the reference is too slow here."""
+    ids = torch.randint(-1, E, (T, k), device="cuda", generator=_gen(T))
+    p = ops.moe_plan(ids, E)
+    flat = ids.reshape(-1)
+    counts = torch.bincount(flat[flat >= 0], minlength=E)
+    offsets = torch.cat([counts.new_zeros(1), ((counts + 15) // 16 * 16).cumsum(0)])
+    order = torch.argsort(flat, stable=True)[int((flat < 0).sum()):]
+    rows = offsets[flat[order]] + torch.arange(order.numel(), device="cuda") - (counts.cumsum(0) - counts)[flat[order]]
+    slots = torch.full_like(flat, -1)
+    slots[order] = rows
+    assert torch.equal(p.counts.long(), counts) and torch.equal(p.offsets.long(), offsets)
+    assert torch.equal(p.slots.reshape(-1).long(), slots)
+    back = torch.full_like(p.rows, -1)
+    back[rows] = order.int()
+    assert torch.equal(p.rows, back)
+
+
 def test_plan_drops_everything_and_takes_far_indices():
     ids = torch.full((9, 2), -1, device="cuda")
     ids[3, 0], ids[4, 1] = 2 ** 40 + 1, -2 ** 50
@@ -323,6 +342,28 @@ def test_captured_training_step():
         want = step()
         g.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_captured_behind_a_joined_side_stream():
+    """The first launch of a call follows two streams at once in the recorded graph."""
+    x, w, ids, ws, res, _ = _inputs(150, 128, 136, 8, 2, 0.0)
+    side = torch.cuda.Stream()
+
+    def step():
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            b = w * 2
+        a = x * 2
+        here.wait_stream(side)
+        with torch.no_grad():
+            return ops.moe_experts(a, b, ids, *ws, residual=res), ops.moe_experts(a[:3], b[:3], ids[:3], *ws)
+
+    g, got = _graph_of(step)
+    x.mul_(0.5)
+    want = step()
+    g.replay()
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
 
 
 def test_streams_run_side_by_side():
