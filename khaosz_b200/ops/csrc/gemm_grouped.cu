@@ -644,23 +644,24 @@ static int moe_sizes(int T, int k, int D, int F, int E, int R) {
   return KB_STATUS_OK;
 }
 
-extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, int w_f32, const int* offsets, const int* slots, const int* rows,
-                                  const int* tiles, int pair, const void* wg, long ldg, long sg, const void* wu, long ldu, long su, const void* wd, long ldd,
-                                  long sd, const void* res, long ldr, void* out, void* xs, float* rw, void* g, void* u, void* h, void* y, int T, int k,
-                                  int D, int F, int E, int R, void* stream) {
+extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, int w_f32, const void* ids, int ids64, int* counts, int* hist,
+                                  int* offsets, int* slots, int* rows, int* tiles, int* pairs, int pair, const void* wg, long ldg, long sg,
+                                  const void* wu, long ldu, long su, const void* wd, long ldd, long sd, const void* res, long ldr, void* out, void* xs,
+                                  float* rw, void* g, void* u, void* h, void* y, int T, int k, int D, int F, int E, int R, void* stream) {
   using namespace kb::grouped;
   KB_TRY(moe_sizes(T, k, D, F, E, R));
   const Weight G{wg, ldg, sg}, U{wu, ldu, su}, W{wd, ldd, sd};
   if (!weight_ok(G, D) || !weight_ok(U, D) || !weight_ok(W, F) || !aligned(x) || (ldx & 7) || (res && (!aligned(res) || (ldr & 7)))) return KB_STATUS_BAD_ARG;
-  if (!aligned(out) || !aligned(xs) || !aligned(g) || !aligned(u) || !aligned(h) || !aligned(y) || !aligned(tiles) || (g == nullptr) != (u == nullptr))
+  if (!aligned(out) || !aligned(xs) || !aligned(g) || !aligned(u) || !aligned(h) || !aligned(y) || !aligned(tiles) || !aligned(pairs) || (g == nullptr) != (u == nullptr))
     return KB_STATUS_BAD_ARG;
   Device d;
   KB_TRY(device(&d));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (ids) KB_TRY(kb_moe_plan(ids, ids64, T * k, E, R, counts, offsets, slots, rows, tiles, pairs, hist, stream));
   KB_TRY(kb::moe::launch_gather(x, ldx, rows, offsets, E, nullptr, weights, w_f32, rw, xs, k, D, R, d.sms, st));
   CUtensorMap a, b, b2;
   Params p{};
-  p.tiles = reinterpret_cast<const int4*>(tiles);
+  p.tiles = reinterpret_cast<const int4*>(pair ? pairs : tiles);
   p.offsets = offsets;
   p.E = E;
   p.err = d.err;

@@ -253,30 +253,25 @@ def moe_plan(experts: Tensor, n_experts: int) -> MoEPlan:
     n, E = experts.numel(), int(n_experts)
     if not experts.is_cuda or n == 0:
         return _plan_torch(experts, E)
-    buf, sizes = _plan_buffer(experts.contiguous(), n, E)
-    tiles, pairs, counts, offsets, slots, rows, *_ = buf.split_with_sizes(sizes)
+    ids = experts.contiguous()
+    words = [z // 4 for z in _plan_sizes(n, E).values()]
+    tiles, pairs, counts, offsets, slots, rows, hist = torch.empty(sum(words), dtype=torch.int32, device=ids.device).split_with_sizes(words)
+    _call(ids, "kb_moe_plan", ids.data_ptr(), ids.dtype == torch.int64, n, E, words[5], counts.data_ptr(), offsets.data_ptr(), slots.data_ptr(),
+          rows.data_ptr(), tiles.data_ptr(), pairs.data_ptr(), hist.data_ptr())
+    _lib.add_launches(_plan_launches(n) - 1)
     return MoEPlan(counts, offsets, slots.view(experts.shape), rows, tiles.view(-1, 4), pairs.view(-1, 4))
 
 
-def _plan_buffer(ids: Tensor, n: int, E: int) -> Tuple[Tensor, list]:
-    """The plan as one int32 buffer: (tiles, pairs, counts, offsets, slots, rows, scratch), of these sizes.  The tiles come
-    first: they are read as 16-byte entries."""
-    R, blocks = rows_bound(n, E), -(-n // PLAN_CHUNK)
-    sizes = [4 * (1 + _tiles_bound(n, E)), 4 * (1 + _tiles_bound(n, E, 2 * TILE_ROWS)), E, E + 1, n, R, (blocks + 1) * E if blocks > 1 else 0]
-    buf = torch.empty(sum(sizes), dtype=torch.int32, device=ids.device)
-    tiles, pairs, counts, offsets, slots, rows, hist = _addresses(buf, sizes)
-    _call(ids, "kb_moe_plan", ids.data_ptr(), ids.dtype == torch.int64, n, E, R, counts, offsets, slots, rows, tiles, pairs, hist)
-    if blocks > 1:
-        _lib.add_launches(2 if blocks >= PLAN_SCAN_FROM else 1)
-    return buf, sizes
+def _plan_sizes(n: int, E: int) -> dict:
+    """Bytes of the plan's arrays.  The tiles come first: they are read as 16-byte entries."""
+    blocks = -(-n // PLAN_CHUNK)
+    return dict(tiles=16 * (1 + _tiles_bound(n, E)), pairs=16 * (1 + _tiles_bound(n, E, 2 * TILE_ROWS)), counts=4 * E, offsets=4 * (E + 1), slots=4 * n,
+                rows=4 * rows_bound(n, E), hist=4 * (blocks + 1) * E if blocks > 1 else 0)
 
 
-def _addresses(buf: Tensor, sizes) -> list:
-    at, out = buf.data_ptr(), []
-    for n in sizes:
-        out.append(at)
-        at += 4 * n
-    return out
+def _plan_launches(n: int) -> int:
+    blocks = -(-n // PLAN_CHUNK)
+    return 1 if blocks == 1 else 2 if blocks < PLAN_SCAN_FROM else 3
 
 
 # ---------------------------------------------------------------------------------------
@@ -344,57 +339,60 @@ def _use_pairs(n: int, E: int) -> bool:
 
 
 class _Space:
-    """One allocation for the scratch of a pass; pieces are 16-byte aligned addresses into it."""
+    """One allocation for the scratch of a pass, in pieces of these sizes, each on a 256-byte boundary."""
 
-    def __init__(self, device, **sizes: int):
+    def __init__(self, device, sizes: dict):
         at, self.offset = 0, {}
         for name, nbytes in sizes.items():
             self.offset[name] = at
-            at += _round_up(nbytes, 256)
+            at += (nbytes + 255) & -256
         self.buf = torch.empty(at, dtype=torch.uint8, device=device)
 
-    def __getitem__(self, name: str):
-        return self.buf.data_ptr() + self.offset[name] if name in self.offset else None
+    def addresses(self, buf: Optional[Tensor] = None) -> dict:
+        base = (self.buf if buf is None else buf).data_ptr()
+        return {name: base + o for name, o in self.offset.items()}
 
 
-def _plan_at(tensors, sizes, pair):
-    """Addresses of (offsets, slots, rows, tiles) in a plan's buffer (with its sizes) or in the tensors of a MoEPlan."""
-    if sizes is None:
-        _, offsets, slots, rows, tiles, pairs = (t.data_ptr() for t in tensors)
-    else:
-        tiles, pairs, _, offsets, slots, rows, _ = _addresses(tensors[0], sizes)
-    return offsets, slots, rows, pairs if pair else tiles
+_PLAN = ("offsets", "slots", "rows", "tiles", "pairs")
 
 
-def _experts_forward(x, weights, residual, plan, sizes, groups, train):
-    """(out, scratch, stacked weights); with ``train`` the scratch keeps what the backward pass reads."""
+def _experts_forward(x, weights, residual, experts, plan, groups, train):
+    """(out, scratch, stacked weights).  The scratch holds the plan too, where none is given, and with ``train`` what the
+    backward pass reads."""
     wg, wu, wd = (_stacked(g) for g in groups)
     (T, D), k, E, F = x.shape, weights.shape[1], wg.shape[0], wg.shape[1]
-    R = rows_bound(T * k, E)
+    n, R = T * k, rows_bound(T * k, E)
     wide, hidden = 2 * R * D, 2 * R * F
-    pair = _use_pairs(T * k, E)
+    sizes = dict(xs=wide, rw=4 * R, h=hidden)
     if train:
-        sp = _Space(x.device, xs=wide, rw=4 * R, h=hidden, g=hidden, u=hidden)
+        sizes.update(g=hidden, u=hidden)
         ys = torch.empty(wide, dtype=torch.uint8, device=x.device)
-        y = ys.data_ptr()
-    else:   # nobody reads the grouped inputs again: the experts' outputs overwrite them
-        sp = _Space(x.device, xs=wide, rw=4 * R, h=hidden)
-        y = sp["xs"]
+    if plan is None:
+        sizes.update(_plan_sizes(n, E))
+    sp = _Space(x.device, sizes)
+    at = sp.addresses()
+    if plan is None:
+        ids = (experts.data_ptr(), experts.dtype == torch.int64, at["counts"], at["hist"])
+    else:
+        ids = (None, 0, None, None)
+        at.update((name, getattr(plan, name).data_ptr()) for name in _PLAN)
     out = torch.empty((T, D), dtype=x.dtype, device=x.device)
-    _call(x, "kb_moe_experts_fwd", x.data_ptr(), x.stride(0), weights.data_ptr(), weights.dtype == torch.float32, *_plan_at(plan, sizes, pair), pair,
-          *_where(wg), *_where(wu), *_where(wd), _p(residual),
-          0 if residual is None else residual.stride(0), out.data_ptr(), sp["xs"], sp["rw"], sp["g"], sp["u"], sp["h"], y, T, k, D, F, E, R)
-    _lib.add_launches(3)
+    # without a backward pass nobody reads the grouped inputs again: the experts' outputs overwrite them
+    _call(x, "kb_moe_experts_fwd", x.data_ptr(), x.stride(0), weights.data_ptr(), weights.dtype == torch.float32, *ids, *(at[name] for name in _PLAN),
+          _use_pairs(n, E), *_where(wg), *_where(wu), *_where(wd), _p(residual), 0 if residual is None else residual.stride(0), out.data_ptr(), at["xs"],
+          at["rw"], at.get("g"), at.get("u"), at["h"], ys.data_ptr() if train else at["xs"], T, k, D, F, E, R)
+    _lib.add_launches(3 + (0 if plan is not None else _plan_launches(n)))
     return out, sp, (wg, wu, wd)
 
 
 class _ExpertsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weights, residual, plan, sizes, n_each, *ws):
+    def forward(ctx, x, weights, residual, experts, plan, n_each, *ws):
         groups = [ws[i * n_each:(i + 1) * n_each] for i in range(3)]
-        out, sp, stacks = _experts_forward(x, weights, residual, plan, sizes, groups, True)
-        ctx.save_for_backward(sp.buf, *stacks, *plan)
-        ctx.space, ctx.sizes, ctx.groups, ctx.n_each, ctx.routing = sp.offset, sizes, groups, n_each, (weights.shape, weights.dtype)
+        out, sp, stacks = _experts_forward(x, weights, residual, experts, plan, groups, True)
+        ctx.save_for_backward(sp.buf, *stacks, *(() if plan is None else plan))
+        ctx.space, ctx.groups, ctx.n_each, ctx.routing = sp, groups, n_each, (weights.shape, weights.dtype)
+        sp.buf = None   # saved above
         for i, w in enumerate(ws):
             if ctx.needs_input_grad[6 + i]:
                 _count_use(w)
@@ -405,11 +403,14 @@ class _ExpertsFn(torch.autograd.Function):
         buf, wg, wu, wd, *plan = ctx.saved_tensors
         ((T, k), w_dtype), (E, F, D), n_each, need = ctx.routing, wg.shape, ctx.n_each, ctx.needs_input_grad
         R = rows_bound(T * k, E)
-        at = {name: buf.data_ptr() + o for name, o in ctx.space.items()}
+        at = ctx.space.addresses(buf)
+        if plan:
+            at.update((name, t.data_ptr()) for name, t in zip(MoEPlan._fields, plan))
         pair = _use_pairs(T * k, E)
         dout = _rows2d(dout)
         dev = dout.device
-        sp = _Space(dev, dys=2 * R * D, dg=2 * R * F, du=2 * R * F, part=4 * R * 2 * -(-F // 256), order=4 * E)
+        sp = _Space(dev, dict(dys=2 * R * D, dg=2 * R * F, du=2 * R * F, part=4 * R * 2 * -(-F // 256), order=4 * E))
+        scratch = sp.addresses()
         dx = torch.empty((T, D), dtype=dout.dtype, device=dev) if need[0] else None
         dw = torch.empty((T, k), dtype=w_dtype, device=dev) if need[1] else None
         mains = [_grad_view(g) for g in ctx.groups] if all(need[6:]) else [None]
@@ -421,7 +422,7 @@ class _ExpertsFn(torch.autograd.Function):
             grads = [torch.empty(w.shape, dtype=w.dtype, device=dev) if wanted else None for w, wanted in ((wg, gate_up), (wu, gate_up), (wd, down))]
         where = [v for g in grads for v in (_where(g) if g is not None else (None, 0, 0))]
         _call(dout, "kb_moe_experts_bwd", dout.data_ptr(), dout.stride(0), at["xs"], at["rw"], at["g"], at["u"], at["h"],
-              *_plan_at(plan, ctx.sizes, pair), pair, *_where(wg), *_where(wu), *_where(wd), sp["dys"], sp["dg"], sp["du"], sp["part"], sp["order"],
+              at["offsets"], at["slots"], at["rows"], at["pairs" if pair else "tiles"], pair, *_where(wg), *_where(wu), *_where(wd), *scratch.values(),
               _p(dx), _p(dw), w_dtype == torch.float32, *where, into, T, k, D, F, E, R)
         _lib.add_launches(1 + (grads[2] is not None) + (dx is not None) + (dx is not None or dw is not None) + (grads[0] is not None))
         out = []
@@ -517,12 +518,9 @@ def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up
     if not train and experts.numel() <= SMALL:
         out = _experts_small(x, weights, experts.contiguous(), residual, *(_stacked(g) for g in groups))
     else:
-        sizes = None
-        if plan is None:
-            buf, sizes = _plan_buffer(experts.contiguous(), experts.numel(), E)
-            plan = (buf,)
+        experts = experts.contiguous()
         if train:
-            out = _ExpertsFn.apply(x, weights, residual, plan, sizes, len(groups[0]), *groups[0], *groups[1], *groups[2])
+            out = _ExpertsFn.apply(x, weights, residual, experts, plan, len(groups[0]), *groups[0], *groups[1], *groups[2])
         else:
-            out = _experts_forward(x, weights, residual, plan, sizes, groups, False)[0]
+            out = _experts_forward(x, weights, residual, experts, plan, groups, False)[0]
     return out if len(shape) == 2 else out.view(shape)
