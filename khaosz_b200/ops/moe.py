@@ -16,6 +16,7 @@ from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import check, lib
@@ -126,6 +127,7 @@ class _RouteFn(torch.autograd.Function):
         return w, ids
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dw, _):
         z, bias, ids = ctx.saved_tensors
         k, sigmoid, _, _, _, renormalize, scale, dtype = ctx.args
@@ -378,8 +380,8 @@ def _experts_forward(x, weights, residual, experts, plan, groups, train):
         at.update((name, getattr(plan, name).data_ptr()) for name in _PLAN)
     out = torch.empty((T, D), dtype=x.dtype, device=x.device)
     # without a backward pass nobody reads the grouped inputs again: the experts' outputs overwrite them
-    _call(x, "kb_moe_experts_fwd", x.data_ptr(), x.stride(0), weights.data_ptr(), weights.dtype == torch.float32, *ids, *(at[name] for name in _PLAN),
-          _use_pairs(n, E), *_where(wg), *_where(wu), *_where(wd), _p(residual), 0 if residual is None else residual.stride(0), out.data_ptr(), at["xs"],
+    _call(x, "kb_moe_experts_fwd", x.data_ptr(), _pitch(x), weights.data_ptr(), weights.dtype == torch.float32, *ids, *(at[name] for name in _PLAN),
+          _use_pairs(n, E), *_where(wg), *_where(wu), *_where(wd), _p(residual), _pitch(residual), out.data_ptr(), at["xs"],
           at["rw"], at.get("g"), at.get("u"), at["h"], ys.data_ptr() if train else at["xs"], T, k, D, F, E, R)
     _lib.add_launches(3 + (0 if plan is not None else _plan_launches(n)))
     return out, sp, (wg, wu, wd)
@@ -399,6 +401,7 @@ class _ExpertsFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         buf, wg, wu, wd, *plan = ctx.saved_tensors
         ((T, k), w_dtype), (E, F, D), n_each, need = ctx.routing, wg.shape, ctx.n_each, ctx.needs_input_grad
@@ -421,7 +424,7 @@ class _ExpertsFn(torch.autograd.Function):
             gate_up, down = any(need[6:6 + 2 * n_each]), any(need[6 + 2 * n_each:])
             grads = [torch.empty(w.shape, dtype=w.dtype, device=dev) if wanted else None for w, wanted in ((wg, gate_up), (wu, gate_up), (wd, down))]
         where = [v for g in grads for v in (_where(g) if g is not None else (None, 0, 0))]
-        _call(dout, "kb_moe_experts_bwd", dout.data_ptr(), dout.stride(0), at["xs"], at["rw"], at["g"], at["u"], at["h"],
+        _call(dout, "kb_moe_experts_bwd", dout.data_ptr(), _pitch(dout), at["xs"], at["rw"], at["g"], at["u"], at["h"],
               at["offsets"], at["slots"], at["rows"], at["pairs" if pair else "tiles"], pair, *_where(wg), *_where(wu), *_where(wd), *scratch.values(),
               _p(dx), _p(dw), w_dtype == torch.float32, *where, into, T, k, D, F, E, R)
         _lib.add_launches(1 + (grads[2] is not None) + (dx is not None) + (dx is not None or dw is not None) + (grads[0] is not None))
@@ -442,8 +445,8 @@ def _experts_small(x, w, ids, res, wg, wu, wd) -> Tensor:
     (T, D), k, (E, F, _) = x.shape, w.shape[1], wg.shape
     out = torch.empty((T, D), dtype=x.dtype, device=x.device)
     h = torch.empty((T * k, F), dtype=torch.float32, device=x.device)
-    _call(x, "kb_moe_experts_small", _p(x), x.stride(0), _p(w), int(w.dtype == torch.float32), _p(ids), int(ids.dtype == torch.int64), *_where(wg), *_where(wu),
-          *_where(wd), _p(res), 0 if res is None else res.stride(0), out.data_ptr(), h.data_ptr(), T, k, D, F, E)
+    _call(x, "kb_moe_experts_small", _p(x), _pitch(x), _p(w), int(w.dtype == torch.float32), _p(ids), int(ids.dtype == torch.int64), *_where(wg), *_where(wu),
+          *_where(wd), _p(res), _pitch(res), out.data_ptr(), h.data_ptr(), T, k, D, F, E)
     _lib.add_launches(1)
     return out
 
@@ -452,7 +455,12 @@ def _rows2d(t: Tensor) -> Tensor:
     """``[rows, D]`` with unit inner stride and a pitch in multiples of 16 bytes."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else t.contiguous()
+    one = t.shape[0] == 1   # its pitch is any number, even where the tensor counts as contiguous: see _pitch
+    return t if t.stride(1) == 1 and (one or t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1]) and t.data_ptr() % 16 == 0 else t.contiguous()
+
+
+def _pitch(t: Optional[Tensor]) -> int:
+    return 0 if t is None else t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _experts_torch(x, weights, ids, wg, wu, wd, residual):
@@ -499,8 +507,8 @@ def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up
         raise ValueError(f"moe_experts: x {tuple(shape)}, weights {tuple(weights.shape)}, experts {tuple(ids_shape)} do not fit [..., {D}], [..., k], [..., k]")
     if residual is not None and residual.shape != shape:
         raise ValueError(f"moe_experts: residual {tuple(residual.shape)} has not the shape of x {tuple(shape)}")
-    every = groups[0] + groups[1] + groups[2] + ((weights, x) if residual is None else (weights, x, residual))
-    if experts.device != x.device or any(t.device != x.device for t in every):
+    wide = groups[0] + groups[1] + groups[2] + ((x,) if residual is None else (x, residual))   # all but the routing weights
+    if experts.device != x.device or weights.device != x.device or any(t.device != x.device for t in wide):
         raise ValueError("moe_experts: all tensors must be on one device")
     if plan is not None and (plan.slots.shape != ids_shape or plan.counts.numel() != E or plan.rows.device != x.device
                              or plan.rows.numel() != rows_bound(experts.numel(), E)):
@@ -511,9 +519,9 @@ def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up
         residual = None if residual is None else residual.reshape(-1, D)
     bf16 = torch.bfloat16
     if (not x.is_cuda or D % 8 or F % 8 or experts.numel() == 0 or weights.dtype not in _KERNEL_DTYPES
-            or any(t.dtype != bf16 for t in every if t is not weights)):
+            or any(t.dtype != bf16 for t in wide)):
         return _experts_torch(x, weights, experts, *(g[0] if lone else g for g in groups), residual).view(shape)
-    train = torch.is_grad_enabled() and any(t.requires_grad for t in every)
+    train = torch.is_grad_enabled() and (weights.requires_grad or any(t.requires_grad for t in wide))
     x, weights, residual = _rows2d(x), weights.contiguous(), None if residual is None else _rows2d(residual)
     if not train and experts.numel() <= SMALL:
         out = _experts_small(x, weights, experts.contiguous(), residual, *(_stacked(g) for g in groups))

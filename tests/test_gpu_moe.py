@@ -237,6 +237,34 @@ def test_experts_layouts(T):
         assert torch.equal(grads[0][:, 2 * D:], dout) and float(grads[0][:, :D].float().abs().max()) == 0
 
 
+@pytest.mark.parametrize("T", [1, 2, 60])
+def test_experts_leading_dimensions_and_single_rows_run_on_the_kernels(T):
+    x, w, ids, ws, res, dout = _inputs(T, 64, 72, 6, 2, 0.0)
+    want = ops.moe_experts(x, w.float(), ids, *ws, residual=res)
+    before = ops.launch_count()
+    lead = lambda t: t.unflatten(0, (1, T))  # noqa: E731
+    assert torch.equal(ops.moe_experts(lead(x), lead(w.float()), lead(ids), *ws, residual=lead(res))[0], want)
+    assert ops.launch_count() > before
+    if T == 1:   # one row of any pitch
+        odd = lambda t: t.reshape(-1, 1).clone().t()  # noqa: E731
+        assert odd(x).stride() == (1, 1)
+        assert torch.equal(ops.moe_experts(odd(x), w.float(), ids, *ws, residual=odd(res)), want)
+        leaf = odd(x).detach().requires_grad_()
+        out = ops.moe_experts(leaf, w, ids, *ws)
+        out.backward(odd(dout))
+        _check({"dx": leaf.grad}, experts_ref(x, w, ids, *ws, dout=dout), ["dx"])
+
+
+def test_second_derivatives_are_refused():
+    x, w, ids, ws, res, dout = _inputs(30, 64, 72, 6, 2, 0.0)
+    x.requires_grad_()
+    z = torch.randn(30, 6, device="cuda", requires_grad=True)
+    for f, leaf in ((lambda: ops.moe_experts(x, w, ids, *ws).float().square().sum(), x), (lambda: ops.moe_route(z, 2)[0].square().sum(), z)):
+        g, = torch.autograd.grad(f(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
 def test_experts_broadcast_gradient_and_frozen_parts():
     x, w, ids, ws, res, dout = _inputs(50, 64, 64, 5, 2, 0.0)
     ref = experts_ref(x, w, ids, *ws, dout=torch.ones_like(dout))
