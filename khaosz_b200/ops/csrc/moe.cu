@@ -79,13 +79,13 @@ struct RouteParams {
 // twice that are in the right order.
 __device__ __forceinline__ float near_score(float c) { return 3e-6f + fabsf(c) * 2.4e-7f; }
 
-// A group's score from its lanes' two largest keys.
+// The two largest keys of a group from its lanes' two largest (the second only where it counts).
 template <typename Key>
-__device__ __forceinline__ Key group_score(Key best, Key next, bool two, int lane) {
-  const Key top = warp_max_key(best);
-  if (!two) return top;
-  if (lane == __ffs(__ballot_sync(FULL, best == top)) - 1) best = next;  // one holder of the largest steps back
-  return key_of(value_of(top) + value_of(warp_max_key(best)));
+__device__ __forceinline__ void group_top(Key best, Key next, bool two, int lane, Key& first, Key& second) {
+  first = warp_max_key(best);
+  if (!two) return;
+  if (lane == __ffs(__ballot_sync(FULL, best == first)) - 1) best = next;  // one holder of the largest steps back
+  second = warp_max_key(best);
 }
 
 // Leaves the keys of the best groups; `close`: the last group taken and the first one left are nearer than the
@@ -97,7 +97,7 @@ __device__ __forceinline__ void only_best_groups(Key (&key)[VPL], const RoutePar
   const bool two = p.group_top == 2 && gs > 1;
   const int per = gs / 32;  // registers of a group
   const bool aligned = per * 32 == gs;
-  Key mine = 0;  // lane g: the key of group g
+  Key mine = 0, and_mine = 0, first, second = 0;  // lane g: the largest keys of group g
   if (aligned) {
     Key best = 0, next = 0;
     int left = per, g = 0;
@@ -108,8 +108,11 @@ __device__ __forceinline__ void only_best_groups(Key (&key)[VPL], const RoutePar
       next = k > best ? best : (k > next ? k : next);
       best = k > best ? k : best;
       if (--left == 0) {
-        const Key score = group_score(best, next, two, lane);
-        if (lane == g) mine = score;
+        group_top(best, next, two, lane, first, second);
+        if (lane == g) {
+          mine = first;
+          and_mine = second;
+        }
         best = next = 0;
         left = per;
         ++g;
@@ -127,10 +130,14 @@ __device__ __forceinline__ void only_best_groups(Key (&key)[VPL], const RoutePar
         next = k > best ? best : (k > next ? k : next);
         best = k > best ? k : best;
       }
-      const Key score = group_score(best, next, two, lane);
-      if (lane == g) mine = score;
+      group_top(best, next, two, lane, first, second);
+      if (lane == g) {
+        mine = first;
+        and_mine = second;
+      }
     }
   }
+  if (two && lane < p.n_groups) mine = key_of(value_of(mine) + value_of(and_mine));
   unsigned keep = 0;
   Key last = 0;
   for (int r = 0; r < p.topk_groups; ++r) {
@@ -187,36 +194,61 @@ __device__ __forceinline__ int take_best(Key (&key)[VPL], const RouteParams& p, 
 }
 
 // The same for fp32 scores.  The low five bits of a key give way to the register's number, which makes a lane's
-// keys unique and the lowest index the largest of equals (the ALU pipe bounds this kernel: fewer compares); the
-// lost bits count as error.  `close`: two neighbours in the ranking, the first expert left behind among them, are
-// within their errors of one another and do not come from the same logit and bias.
+// keys unique and the lowest index the largest of equals; the lost bits count as error.  Unique keys need no
+// payload: each lane sorts its own, and a round takes the largest of the 32 heads and shifts one lane's list (the
+// ALU pipe bounds this kernel; rounds that searched all registers took a fifth longer).  `close`: two neighbours in
+// the ranking, the first expert left behind among them, are within their errors of one another and do not come
+// from the same logit and bias.
 constexpr unsigned NUMBER = 31u;
 __device__ __forceinline__ float near_key(float c) { return near_score(c) + fabsf(c) * 7.7e-6f; }  // 2^-17 and a bit
+template <int N>
+__device__ __forceinline__ void sort_falling(uint32_t (&v)[N]) {  // bitonic network
+#pragma unroll
+  for (int k = 2; k <= N; k *= 2) {
+#pragma unroll
+    for (int j = k / 2; j > 0; j /= 2) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int o = i ^ j;
+        if (o < i) continue;
+        const uint32_t hi = max(v[i], v[o]), lo = min(v[i], v[o]);
+        v[i] = i & k ? lo : hi;
+        v[o] = i & k ? hi : lo;
+      }
+    }
+  }
+}
 template <int VPL, typename T>
 __device__ __forceinline__ int take_best_scored(uint32_t (&key)[VPL], const RouteParams& p, const T* zrow, int lane, bool& close) {
 #pragma unroll
   for (int i = 0; i < VPL; ++i) key[i] = key[i] ? (key[i] & ~NUMBER) | (NUMBER - i) : 0u;
-  int mine = 0, prev_e = 0;
-  float prev = 0.f;
+  sort_falling(key);
+  uint32_t mine_key = 0u, last_key = 0u;
+  int mine = 0, last = 0;
   const int rounds = p.k < p.E ? p.k + 1 : p.k;
   for (int j = 0; j < rounds; ++j) {
-    uint32_t best = key[0];
+    last_key = __reduce_max_sync(FULL, key[0]);
+    const int who = __ffs(__ballot_sync(FULL, key[0] == last_key)) - 1;
+    last = (int)(NUMBER - (last_key & NUMBER)) * 32 + who;
+    if (lane == j) {
+      mine = last;
+      mine_key = last_key;
+    }
+    const bool shift = lane == who;
 #pragma unroll
-    for (int i = 1; i + 1 < VPL; i += 2) best = __vimax3_u32(best, key[i], key[i + 1]);
-    if (VPL % 2 == 0) best = max(best, key[VPL - 1]);
-    const uint32_t top = __reduce_max_sync(FULL, best);
-    if (top == 0) break;  // nothing is left to be chosen
-    const int who = __ffs(__ballot_sync(FULL, best == top)) - 1;
-    const uint32_t gone = lane == who ? top : 1u;  // no key is 1
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) key[i] = key[i] == gone ? 0u : key[i];
-    const int e = (int)(NUMBER - (top & NUMBER)) * 32 + who;
-    if (lane == j) mine = e;
-    const float c = value_of(top & ~NUMBER);
-    if (j && !(prev - c > near_key(prev)) && c > -3e38f)
-      close |= !(to_f(zrow[e]) == to_f(zrow[prev_e]) && (!p.bias || p.bias[e] == p.bias[prev_e]));
-    prev = c;
-    prev_e = e;
+    for (int i = 0; i + 1 < VPL; ++i) key[i] = shift ? key[i + 1] : key[i];
+    key[VPL - 1] = shift ? 0u : key[VPL - 1];
+  }
+  // each slot against the one behind it; lane 31 finds the 33rd in `last`
+  uint32_t next_key = __shfl_down_sync(FULL, mine_key, 1);
+  int next = __shfl_down_sync(FULL, mine, 1);
+  if (lane == 31) {
+    next_key = rounds == 33 ? last_key : 0u;
+    next = last;
+  }
+  if (next_key != 0u) {  // 0: nothing was left to be chosen
+    const float c = value_of(mine_key & ~NUMBER), d = value_of(next_key & ~NUMBER);
+    if (!(c - d > near_key(c)) && d > -3e38f) close = !(to_f(zrow[mine]) == to_f(zrow[next]) && (!p.bias || p.bias[mine] == p.bias[next]));
   }
   return mine;
 }
@@ -279,37 +311,47 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(const RouteParams p) {
   if (t >= p.T) return;
   const T* zrow = static_cast<const T*>(p.z) + (size_t)t * p.ldz;
   float z[VPL];
-  bool bad = false;
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
-    const int e = i * 32 + lane;
-    z[i] = e < p.E ? to_f(zrow[e]) : -INFINITY;
-    bad |= isnan(z[i]) || (!p.sigmoid && z[i] == INFINITY);
+    z[i] = i * 32 + lane < p.E ? to_f(zrow[i * 32 + lane]) : -INFINITY;
     m = fmaxf(m, z[i]);
   }
-  float b[VPL];
-  if constexpr (SCORED) {
+  // A NaN shows in the sum of the scores (for the softmax plus infinity too), or is looked for where none is formed.
+  bool bad = false;
+  float row_sum = 1.f;
+  float c[SCORED ? VPL : 1];
+  if (!p.sigmoid) m = warp_max(m);
+  if (SCORED || (!p.sigmoid && !p.renorm)) {
+    row_sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      b[i] = p.bias && i * 32 + lane < p.E ? __ldg(p.bias + i * 32 + lane) : 0.f;
-      bad |= isnan(b[i]);
+      const float s = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-z[i])) : (z[i] == -INFINITY ? 0.f : __expf(z[i] - m));
+      row_sum += s;
+      if constexpr (SCORED) c[i] = s;
+    }
+    row_sum = warp_sum(row_sum);
+    bad = isnan(row_sum);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) bad |= z[i] != z[i];
+    bad |= !p.sigmoid && m == INFINITY;
+  }
+  if constexpr (SCORED) {
+    const float inv = p.sigmoid ? 1.f : (row_sum > 0.f ? 1.f / row_sum : 0.f);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const float b = p.bias && i * 32 + lane < p.E ? __ldg(p.bias + i * 32 + lane) : 0.f;
+      bad |= b != b;
+      c[i] = z[i] == -INFINITY ? -INFINITY : fmaf(c[i], inv, b);
     }
   }
-  if (!p.sigmoid) m = warp_max(m);
   if (__any_sync(FULL, bad)) {  // no distribution: valid indices, weights that show it
     if (lane < p.k) {
       p.ids[(size_t)t * p.k + lane] = lane;
       store_f(p.w, (size_t)t * p.k + lane, p.w_f32, NAN);
     }
     return;
-  }
-  float row_sum = 1.f;
-  if (!p.sigmoid && (SCORED || !p.renorm)) {
-    row_sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) row_sum += z[i] == -INFINITY ? 0.f : __expf(z[i] - m);
-    row_sum = warp_sum(row_sum);
   }
   uint32_t key[VPL];
   bool close = false;
@@ -323,13 +365,8 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(const RouteParams p) {
     }
     mine = take_best(key, p, lane);
   } else {
-    const float inv = row_sum > 0.f ? 1.f / row_sum : 0.f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      float c = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-z[i])) : __expf(z[i] - m) * inv;
-      c = z[i] == -INFINITY ? -INFINITY : c + b[i];
-      key[i] = i * 32 + lane < p.E ? key_of(c) : 0u;
-    }
+    for (int i = 0; i < VPL; ++i) key[i] = i * 32 + lane < p.E ? key_of(c[i]) : 0u;
     if (p.n_groups > 1) {
       only_best_groups(key, p, lane, close);
       if (!p.bias) {  // inside the groups the logits tell the order
@@ -338,8 +375,9 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(const RouteParams p) {
           if (key[i]) key[i] = key_of(z[i]);
       }
     }
-    mine = p.bias ? take_best_scored(key, p, zrow, lane, close) : take_best(key, p, lane);
-    if (close) mine = rank_wide<VPL, T>(p, zrow, lane, m);  // uniform in the warp
+    bool near = false;
+    mine = p.bias ? take_best_scored(key, p, zrow, lane, near) : take_best(key, p, lane);
+    if (__any_sync(FULL, close || near)) mine = rank_wide<VPL, T>(p, zrow, lane, m);
   }
   const bool slot = lane < p.k;
   const float zs = slot ? to_f(zrow[mine]) : -INFINITY;
