@@ -661,8 +661,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const __nv_bfloat16* src, l
       for (int c = lane; c < D / 8; c += 32) o[c] = make_uint4(0u, 0u, 0u, 0u);
     } else {
       const uint4* s = reinterpret_cast<const uint4*>(src + (size_t)(a / k) * ld);
-#pragma unroll 4
-      for (int c = lane; c < D / 8; c += 32) o[c] = s[c];
+#pragma unroll 8
+      for (int c = lane; c < D / 8; c += 32) o[c] = __ldg(s + c);
     }
     if (rw && lane == 0) rw[r] = a < 0 ? 0.f : load_f(w, a, w_f32);
   }
@@ -686,10 +686,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, co
       float acc[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+#pragma unroll 4
       for (int j = 0; j < k; ++j) {
         const int r = sl[j];
-        if (r < 0) continue;
-        const uint4 v = *reinterpret_cast<const uint4*>(y + (size_t)r * D + c * 8);
+        const uint4 v = r < 0 ? make_uint4(0u, 0u, 0u, 0u) : __ldg(reinterpret_cast<const uint4*>(y + (size_t)r * D + c * 8));
         const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), d = unpack_bf16x2(v.z), f = unpack_bf16x2(v.w);
         acc[0] += a.x; acc[1] += a.y; acc[2] += b.x; acc[3] += b.y;
         acc[4] += d.x; acc[5] += d.y; acc[6] += f.x; acc[7] += f.y;
