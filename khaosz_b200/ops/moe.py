@@ -95,11 +95,12 @@ def _route_torch(z, bias, k, sigmoid, n_groups, topk_groups, group_top, renormal
         e = torch.exp(zf - top.masked_fill(top == -torch.inf, 0.0))
         total = e.sum(-1, keepdim=True)
         w = (e / total.masked_fill(total == 0, 1.0)).gather(1, ids)
-    elif sigmoid:
+    elif not renormalize:
         w = torch.sigmoid(picked)
-    else:
-        top = picked.detach().masked_fill(off, -torch.inf).amax(-1, keepdim=True)
-        w = torch.exp(picked.masked_fill(off, -torch.inf) - top.masked_fill(top == -torch.inf, 0.0))
+    else:   # ratios of scores, which hold where the scores themselves are too small to be told from zero
+        log = (torch.nn.functional.logsigmoid(picked) if sigmoid else picked).masked_fill(off, -torch.inf)
+        top = log.detach().amax(-1, keepdim=True)
+        w = torch.exp(log - top.masked_fill(top == -torch.inf, 0.0))
     w = w.masked_fill(off, 0.0)
     if renormalize:
         total = w.sum(-1, keepdim=True)
@@ -150,7 +151,8 @@ def moe_route(logits: Tensor, k: int, *, score: str = "softmax", bias: Optional[
     ``renormalize``, times ``scale``, in ``dtype`` (default: that of the logits).
 
     A logit or a bias of minus infinity disables an expert: it is chosen only where no other is left and has weight 0, so a row
-    of nothing else has weights 0.  A row with a NaN (for the softmax also with plus infinity) has weights NaN and the experts
+    of nothing else has weights 0.  Any finite logit is a score like others: renormalised weights keep the ratios of scores that
+    are too small to be represented (a row of the type's lowest value has equal weights).  A row with a NaN (for the softmax also with plus infinity) has weights NaN and the experts
     ``0..k-1``.  Supports up to 1024 experts, 32 groups and ``k <= 32``.
     """
     if logits.dim() < 1 or not logits.is_floating_point():

@@ -61,7 +61,9 @@ def test_route_special_rows_and_layouts():
             w, ids = ops.moe_route(z, 4, score=score, bias=bias)
             assert torch.isnan(w[1]).all() and (torch.isnan(w[2]).all() == (score == "softmax"))
             assert ids[[0, 1, 4]].tolist() == [[0, 1, 2, 3]] * 3
-            assert torch.allclose(w[[0, 4]], torch.full((2, 4), 0.25, device="cuda"))
+            assert torch.allclose(w[[0, 3, 4]], torch.full((3, 4), 0.25, device="cuda"))
+    tiny = torch.tensor([[-200.0, -201.0, -300.0]], device="cuda")   # the scores are zero in fp32, their ratios are not
+    assert torch.allclose(ops.moe_route(tiny, 2, score="sigmoid")[0], torch.softmax(tiny[:, :2], -1), rtol=1e-5)
     bias = torch.zeros(40, device="cuda")
     bias[:38] = -torch.inf   # two experts are left for four slots
     w, ids = ops.moe_route(z, 4, bias=bias)

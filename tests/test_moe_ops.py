@@ -52,7 +52,10 @@ def test_route_ties_go_to_the_lowest_index_and_nan_rows_show():
     w, ids = ops.moe_route(z, 3)
     assert ids.tolist() == [[0, 1, 2]] * 3
     assert torch.isnan(w[1]).all() and torch.allclose(w[[0, 2]], torch.full((2, 3), 1 / 3))
-    assert torch.isnan(ops.moe_route(z, 3, score="sigmoid")[0][1]).all()
+    w = ops.moe_route(z, 3, score="sigmoid")[0]
+    assert torch.isnan(w[1]).all() and torch.allclose(w[[0, 2]], torch.full((2, 3), 1 / 3))
+    tiny = torch.tensor([[-200.0, -201.0, -300.0]])   # the scores are zero in fp32, their ratios are not
+    assert torch.allclose(ops.moe_route(tiny, 2, score="sigmoid")[0], torch.softmax(tiny[:, :2], -1))
 
 
 def test_route_refuses():
