@@ -17,6 +17,11 @@
 // once, in the epilogue.  In the weight gradients K runs over an expert's rows in steps of 16, the alignment of
 // its segment, whose padding rows are zero.  All waits are bounded (common.cuh).
 //
+// What a product hands on is bf16 where a tensor core reads it next (h, dG, dU).  What only arithmetic reads, the
+// projections that the backward pass needs and the experts' output and input-gradient rows before they are added up,
+// is fp16 with a power of two for every 32 columns of a row (moe.cuh): eight times the precision of bf16 in the same
+// 16 bits, whatever the magnitude.
+//
 // Two forms.  A single CTA per tile reads (128 + 256) x 64 operands per K block: 92 bytes per clock at the tensor
 // cores' full rate, more than the about 64 that reach an SM from L2, and that bounds it (13 to 15 TB/s measured).
 // PAIR: two CTAs of a cluster compute 256 x 256 together (tcgen05 cta_group::2), each staging its own 128 rows
@@ -59,7 +64,9 @@ struct Params {
   int M, N;             // valid rows of a weight gradient; valid columns
   __nv_bfloat16 *out0, *out1, *out2;
   long ld0, ld1, stride0, stride1;  // pitch and (weight gradients) distance of the experts
-  const __nv_bfloat16 *g, *u;       // DHID: [rows, N]
+  const __nv_bfloat16 *g, *u;       // DHID: [rows, N] fp16 blocks
+  __nv_bfloat16 *s0, *s1;           // factors of the fp16 blocks: of out0 and out1, DX and DOWN of out0, DHID of g and u
+  int sld;                          // their pitch
   const float* rw;                  // GATE_UP, DHID: routing weight of a row
   float* part;                      // DHID: [rows, 2 num_n]
   int accumulate;                   // weight gradients: add to what is there
@@ -408,7 +415,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       const size_t row0 = t.row0 + q * 32;
       const int rows = min(32, t.end - (t.row0 + q * 32));
       uint4 vg[4], vu[4];
+      float kg = 0.f, ku = 0.f;  // this lane's row's factors of the columns under way
       auto fetch = [&](int c) {
+        if (t.row0 + row < t.end && t.n0 + c * 32 < p.N) {
+          const size_t at = (size_t)(t.row0 + row) * p.sld + t.n0 / 32 + c;
+          kg = __bfloat162float(p.s0[at]);
+          ku = __bfloat162float(p.s1[at]);
+        }
         const int col = t.n0 + c * 32 + c4 * 8;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -437,6 +450,15 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
               tmem_ld_32x32b_x32(t_row + c * 32, vg);
               tmem_ld_32x32b_x32(t_row + BN / 2 + c * 32, vu);
               tmem_ld_wait();
+              float kg = 0.f, ku = 0.f, back_g = 0.f, back_u = 0.f;
+              if (p.out0) {
+                kg = kb::moe::block_factor(vg, back_g);
+                ku = kb::moe::block_factor(vu, back_u);
+                if (live) {
+                  p.s0[grow * p.sld + col / 32] = __float2bfloat16(back_g);
+                  p.s1[grow * p.sld + col / 32] = __float2bfloat16(back_u);
+                }
+              }
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 float g[8], u[8], h[8];
@@ -449,8 +471,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                 if (live && col + i * 8 < p.N) {
                   *reinterpret_cast<uint4*>(p.out2 + grow * p.ld0 + col + i * 8) = pack8(h);
                   if (p.out0) {
-                    *reinterpret_cast<uint4*>(p.out0 + grow * p.ld0 + col + i * 8) = pack8(g);
-                    *reinterpret_cast<uint4*>(p.out1 + grow * p.ld0 + col + i * 8) = pack8(u);
+                    *reinterpret_cast<uint4*>(p.out0 + grow * p.ld0 + col + i * 8) = kb::moe::pack_block8(g, kg);
+                    *reinterpret_cast<uint4*>(p.out1 + grow * p.ld0 + col + i * 8) = kb::moe::pack_block8(u, ku);
                   }
                 }
               }
@@ -467,6 +489,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                 *reinterpret_cast<uint4*>(su + staged(r, c4)) = vu[i];
               }
               __syncwarp();
+              const float fg = kg, fu = ku;
               if (c + 1 < chunk0 + CHUNKS && t.n0 + (c + 1) * 32 < p.N) fetch(c + 1);  // under way during the arithmetic
               uint32_t v[32];
               tmem_ld_32x32b_x32(t_row + c * 32, v);
@@ -476,8 +499,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                 uint4* pg = reinterpret_cast<uint4*>(sg + staged(lane, i));
                 uint4* pu = reinterpret_cast<uint4*>(su + staged(lane, i));
                 float g[8], u[8], dg[8], du[8];
-                unpack8(*pg, g);
-                unpack8(*pu, u);
+                kb::moe::unpack_block8(*pg, fg, g);
+                kb::moe::unpack_block8(*pu, fu, u);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
                   const float d = __uint_as_float(v[i * 8 + x]), s = sigmoid(g[x]), act = g[x] * s, da = d * act;
@@ -509,10 +532,16 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
               uint32_t v[32];
               tmem_ld_32x32b_x32(t_row + c * 32, v);
               tmem_ld_wait();
+              float back;
+              const float k = kb::moe::block_factor(v, back);
+              if (live) p.s0[grow * p.sld + col / 32] = __float2bfloat16(back);
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (live && col + i * 8 < p.N)
-                  *reinterpret_cast<uint4*>(p.out0 + grow * p.ld0 + col + i * 8) = pack8(reinterpret_cast<const float*>(v + i * 8));
+              for (int i = 0; i < 4; ++i) {
+                float f[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(v[i * 8 + x]);
+                if (live && col + i * 8 < p.N) *reinterpret_cast<uint4*>(p.out0 + grow * p.ld0 + col + i * 8) = kb::moe::pack_block8(f, k);
+              }
             }
           }
         }
@@ -675,6 +704,11 @@ extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, 
   p.out1 = static_cast<__nv_bfloat16*>(u);
   p.out2 = static_cast<__nv_bfloat16*>(h);
   p.ld0 = F;
+  p.sld = cdiv(F, 32);
+  if (g) {
+    p.s0 = p.out0 + (size_t)R * F;  // the factors lie behind the values
+    p.s1 = p.out1 + (size_t)R * F;
+  }
   p.rw = rw;
   KB_TRY(launch<GATE_UP>(pair, a, a, b, b2, p, d.dev, d.sms, st));
   KB_TRY(rows_map(&a, h, R, F, BM));
@@ -685,8 +719,10 @@ extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, 
   p.out0 = static_cast<__nv_bfloat16*>(y);
   p.out1 = p.out2 = nullptr;
   p.ld0 = D;
+  p.sld = cdiv(D, 32);
+  p.s0 = p.out0 + (size_t)R * D;
   KB_TRY(launch<DOWN>(pair, a, a, b, b, p, d.dev, d.sms, st));
-  return kb::moe::launch_combine(y, slots, res, ldr, out, nullptr, 0, nullptr, 0, T, k, D, st);
+  return kb::moe::launch_combine(y, slots, res, ldr, out, nullptr, 0, nullptr, 0, T, k, D, R, st);
 }
 
 extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, const float* rw, const void* g, const void* u, const void* h,
@@ -725,6 +761,9 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
   p.ld0 = F;
   p.g = static_cast<const __nv_bfloat16*>(g);
   p.u = static_cast<const __nv_bfloat16*>(u);
+  p.s0 = const_cast<__nv_bfloat16*>(p.g) + (size_t)R * F;
+  p.s1 = const_cast<__nv_bfloat16*>(p.u) + (size_t)R * F;
+  p.sld = cdiv(F, 32);
   p.rw = rw;
   p.part = part;
   KB_TRY(launch<DHID>(pair, a, a, b, b, p, d.dev, d.sms, st));
@@ -753,9 +792,11 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
     p.N = D;
     p.out0 = static_cast<__nv_bfloat16*>(dys);
     p.ld0 = D;
+    p.s0 = p.out0 + (size_t)R * D;
+    p.sld = cdiv(D, 32);
     KB_TRY(launch<DX>(pair, a, a2, b, b2, p, d.dev, d.sms, st));
   }
-  if (dx || dw) KB_TRY(kb::moe::launch_combine(dys, slots, nullptr, 0, dx, part, n_part, dw, w_f32, T, k, D, st));
+  if (dx || dw) KB_TRY(kb::moe::launch_combine(dys, slots, nullptr, 0, dx, part, n_part, dw, w_f32, T, k, D, R, st));
   if (dwg) {
     KB_TRY(rows_map(&a, dg, R, F, BK));
     KB_TRY(rows_map(&a2, du, R, F, BK));

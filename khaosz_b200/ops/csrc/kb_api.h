@@ -219,8 +219,8 @@ int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int* counts, in
                 int* hist, void* stream);
 // out = res + the experts' products, with the arrays of a plan (with `pair` two CTAs share a tile, of its pairs) or, where ids is
 // given, grouping them first into these arrays (counts and hist are not read otherwise); the weights [E, F, D], [E, F, D], [E, D, F]
-// (pitch, distance of the experts); scratch: xs [R,D], rw [R], h [R,F], y [R,D] (may be xs); g, u [R,F] (both or neither) keep the
-// projections for the backward pass.
+// (pitch, distance of the experts); scratch: xs [R,D], rw [R], h [R,F], y (may be xs); g, u (both or neither) keep the projections for the
+// backward pass.  y, g, u are fp16 blocks: [R, cols] and behind them a bf16 factor for every 32 columns, [R, ceil(cols / 32)].
 int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, int w_f32, const void* ids, int ids64, int* counts, int* hist, int* offsets,
                        int* slots, int* rows, int* tiles, int* pairs, int pair, const void* wg, long ldg, long sg, const void* wu, long ldu,
                        long su, const void* wd, long ldd, long sd, const void* res, long ldr, void* out, void* xs, float* rw, void* g, void* u,
@@ -230,7 +230,7 @@ int kb_moe_experts_small(const void* x, long ldx, const void* weights, int w_f32
                          const void* wu, long ldu, long su, const void* wd, long ldd, long sd, const void* res, long ldr, void* out, float* h,
                          int T, int k, int D, int F, int E, void* stream);
 // Backward pass (tiles: the plan's tiles, or its pairs with `pair`): dx [T,D], dw [T,k] and the weights' gradients, each optional (dwg and dwu together); accumulate: the weights' gradients are
-// added to what is there.  Scratch: dys [R,D], dg, du [R,F], part [R, 2 ceil(F / 256)], order [E].
+// added to what is there.  Scratch: dys (fp16 blocks of D columns), dg, du [R,F], part [R, 2 ceil(F / 256)], order [E].
 int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, const float* rw, const void* g, const void* u, const void* h,
                        const int* offsets, const int* slots, const int* rows, const int* tiles, int pair, const void* wg, long ldg, long sg, const void* wu,
                        long ldu, long su, const void* wd, long ldd, long sd, void* dys, void* dg, void* du, float* part, int* order, void* dx, void* dw,

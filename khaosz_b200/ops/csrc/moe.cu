@@ -668,9 +668,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const __nv_bfloat16* src, l
   }
 }
 
-// out[t] = residual[t] + sum_j y[slots[t][j]] in fp32, rounded once; a dropped slot adds nothing.
+// out[t] = residual[t] + sum_j y[slots[t][j]] in fp32, rounded once; a dropped slot adds nothing.  y is in fp16 blocks.
 // With `part`: dweights[t][j] = sum over the feature tiles of its row's partial dot products.
-__global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, const int* slots, const __nv_bfloat16* res, long ldr, __nv_bfloat16* out,
+__global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, const __nv_bfloat16* factors, const int* slots, const __nv_bfloat16* res, long ldr, __nv_bfloat16* out,
                                                       const float* part, int n_part, void* dw, int w_f32, int T, int k, int D) {
   await_predecessor();
   const int per = D / 8;
@@ -681,6 +681,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, co
   const int t = blockIdx.x * groups + g;
   if (t >= T) return;
   const int* sl = slots + (size_t)t * k;
+  const int blocks = (D + 31) / 32;
   if (out) {
     for (int c = c0; c < per; c += lanes) {
       float acc[8];
@@ -689,10 +690,16 @@ __global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, co
 #pragma unroll 4
       for (int j = 0; j < k; ++j) {
         const int r = sl[j];
-        const uint4 v = r < 0 ? make_uint4(0u, 0u, 0u, 0u) : __ldg(reinterpret_cast<const uint4*>(y + (size_t)r * D + c * 8));
-        const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), d = unpack_bf16x2(v.z), f = unpack_bf16x2(v.w);
-        acc[0] += a.x; acc[1] += a.y; acc[2] += b.x; acc[3] += b.y;
-        acc[4] += d.x; acc[5] += d.y; acc[6] += f.x; acc[7] += f.y;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        float back = 0.f;
+        if (r >= 0) {
+          v = __ldg(reinterpret_cast<const uint4*>(y + (size_t)r * D + c * 8));
+          back = __bfloat162float(factors[(size_t)r * blocks + c / 4]);
+        }
+        float f[8];
+        unpack_block8(v, back, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += f[i];
       }
       if (res) {
         const uint4 v = *reinterpret_cast<const uint4*>(res + (size_t)t * ldr + c * 8);
@@ -819,9 +826,10 @@ int launch_gather(const void* src, long ld, const int* rows, const int* offsets,
 }
 
 int launch_combine(const void* y, const int* slots, const void* res, long ldr, void* out, const float* part, int n_part, void* dw, int w_f32, int T, int k,
-                   int D, cudaStream_t st) {
+                   int D, int R, cudaStream_t st) {
   const int per = D / 8, lanes = per < 256 ? per : 256, groups = 256 / lanes;
-  launch_after(combine_kernel, (T + groups - 1) / groups, 256, 0, st, static_cast<const __nv_bfloat16*>(y), slots,
+  launch_after(combine_kernel, (T + groups - 1) / groups, 256, 0, st, static_cast<const __nv_bfloat16*>(y),
+               static_cast<const __nv_bfloat16*>(y) + (size_t)R * D, slots,
                static_cast<const __nv_bfloat16*>(res), ldr, static_cast<__nv_bfloat16*>(out), part, n_part, dw, w_f32, T, k, D);
   return launched();
 }

@@ -1,6 +1,8 @@
 // Passes of moe.cu that gemm_grouped.cu runs around its products.
 #pragma once
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <stdint.h>
 
 namespace kb {
 namespace moe {
@@ -31,13 +33,44 @@ cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, size_
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// fp16 blocks: 32 columns of a row share a power of two, kept as bf16 behind the [R, cols] values ([R, ceil(cols / 32)]),
+// that brings the largest of them to 2^14..2^15: 11 bits for everything down to 2^-28 of it.
+// The factor before rounding, from the 32 fp32 accumulators; `back`: its inverse.  An infinity or a NaN stays one.
+__device__ __forceinline__ float block_factor(const uint32_t (&v)[32], float& back) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) m = max(m, v[i] & 0x7fffffffu);
+  const uint32_t e = min(max(m >> 23, 15u), 254u);
+  back = __uint_as_float((e - 14u) << 23);
+  return __uint_as_float((268u - e) << 23);
+}
+__device__ __forceinline__ uint4 pack_block8(const float* f, float k) {
+  uint4 o;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(f[2 * i] * k, f[2 * i + 1] * k);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return o;
+}
+__device__ __forceinline__ void unpack_block8(const uint4& v, float back, float* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = h.x * back;
+    f[2 * i + 1] = h.y * back;
+  }
+}
+
 // dst[r] = src[rows[r] / k] for the first offsets[E] rows (zero where rows[r] < 0); rw[r]: the row's routing weight (may be
 // null); order (may be null): the experts by falling number of rows.
 int launch_gather(const void* src, long ld, const int* rows, const int* offsets, int E, int* order, const void* w, int w_f32, float* rw, void* dst, int k, int D, int R, int sms,
                   cudaStream_t st);
-// out[t] = res[t] + sum_j y[slots[t][j]] (out may be null); dw[t][j] = sum_i part[slots[t][j]][i] (dw may be null).
+// out[t] = res[t] + sum_j y[slots[t][j]] with y [R, D] in fp16 blocks (out may be null); dw[t][j] = sum_i part[slots[t][j]][i] (dw may be null).
 int launch_combine(const void* y, const int* slots, const void* res, long ldr, void* out, const float* part, int n_part, void* dw, int w_f32, int T, int k,
-                   int D, cudaStream_t st);
+                   int D, int R, cudaStream_t st);
 
 }  // namespace moe
 }  // namespace kb

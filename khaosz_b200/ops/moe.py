@@ -357,6 +357,11 @@ class _Space:
         return {name: base + o for name, o in self.offset.items()}
 
 
+def _blocks_bytes(rows: int, cols: int) -> int:
+    """``[rows, cols]`` in fp16, and behind it a bf16 factor for every 32 columns of a row."""
+    return 2 * rows * (cols + -(-cols // 32))
+
+
 _PLAN = ("offsets", "slots", "rows", "tiles", "pairs")
 
 
@@ -366,10 +371,10 @@ def _experts_forward(x, weights, residual, experts, plan, groups, train):
     wg, wu, wd = (_stacked(g) for g in groups)
     (T, D), k, E, F = x.shape, weights.shape[1], wg.shape[0], wg.shape[1]
     n, R = T * k, rows_bound(T * k, E)
-    wide, hidden = 2 * R * D, 2 * R * F
-    sizes = dict(xs=wide, rw=4 * R, h=hidden)
+    wide = _blocks_bytes(R, D)
+    sizes = dict(xs=wide, rw=4 * R, h=2 * R * F)
     if train:
-        sizes.update(g=hidden, u=hidden)
+        sizes.update(g=_blocks_bytes(R, F), u=_blocks_bytes(R, F))
         ys = torch.empty(wide, dtype=torch.uint8, device=x.device)
     if plan is None:
         sizes.update(_plan_sizes(n, E))
@@ -414,7 +419,7 @@ class _ExpertsFn(torch.autograd.Function):
         pair = _use_pairs(T * k, E)
         dout = _rows2d(dout)
         dev = dout.device
-        sp = _Space(dev, dict(dys=2 * R * D, dg=2 * R * F, du=2 * R * F, part=4 * R * 2 * -(-F // 256), order=4 * E))
+        sp = _Space(dev, dict(dys=_blocks_bytes(R, D), dg=2 * R * F, du=2 * R * F, part=4 * R * 2 * -(-F // 256), order=4 * E))
         scratch = sp.addresses()
         dx = torch.empty((T, D), dtype=dout.dtype, device=dev) if need[0] else None
         dw = torch.empty((T, k), dtype=w_dtype, device=dev) if need[1] else None
@@ -488,8 +493,8 @@ def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up
     experts, where it is at hand.  Gradients reach ``x``, ``weights``, ``residual`` and the experts' matrices, whose
     ``main_grad`` buffers receive them in place; an expert without tokens gets zeros.
 
-    The kernels take CUDA bf16 with D and F in multiples of 8 (weights also fp32); sums are held in fp32 and rounded once,
-    the hidden activations and each expert's output row are bf16.
+    The kernels take CUDA bf16 with D and F in multiples of 8 (weights also fp32); sums are held in fp32, the hidden activations
+    and their gradients are rounded to bf16 before the next product, what else is kept between the passes has 11 bits.
     """
     lone = isinstance(w_gate, Tensor)
     if any(isinstance(w, Tensor) != lone for w in (w_up, w_down)):

@@ -2,6 +2,7 @@
 import torch
 
 U = 2.0 ** -8       # half a step of bf16, relative
+UH = 2.0 ** -11     # half a step of fp16, relative (the kernels' blocks of 32 keep it down to 2^-28 of the block's largest)
 U32 = 2.0 ** -23    # one step of fp32, relative
 
 
@@ -70,8 +71,9 @@ def plan(ids, E, align=16):
 
 def experts(x, w, ids, wg, wu, wd, residual=None, dout=None):
     """{"out", "dx", "dw", "dgate", "dup", "ddown"}: (value in 64 bits, elementwise bound) of bf16 kernels that keep sums in
-    fp32, round the hidden activations, each expert's output row and the results to bf16, and in the backward pass start
-    from projections that were rounded to bf16.  Every bound adds half a step per rounding, carried through the following
+    fp32, round the hidden activations, their gradients and the results to bf16 and each expert's output and input-gradient
+    row to fp16, and in the backward pass start from projections that were rounded to fp16 (absolute errors of a block's
+    smallest values, 2^-39 of its largest, are far below the fp32 steps of the sums).  Every bound adds half a step per rounding, carried through the following
     product by absolute values, and one fp32 step per summand of a product."""
     dev = x.device
     X, W = x.detach().double(), w.detach().double()
@@ -95,13 +97,13 @@ def experts(x, w, ids, wg, wu, wd, residual=None, dout=None):
         y = h @ Wd[e].T
         ey = eh @ Wd[e].T.abs() + F * U32 * (h.abs() @ Wd[e].T.abs())
         out.index_add_(0, t, y)
-        e_out.index_add_(0, t, ey + U * (y.abs() + ey))
+        e_out.index_add_(0, t, ey + UH * (y.abs() + ey))
         if dout is None:
             continue
         do = dout.detach().double()[t]
         dh = do @ Wd[e]
         edh = D * U32 * (do.abs() @ Wd[e].abs())
-        eg, eu = eg + U * (g.abs() + eg), eu + U * (u.abs() + eu)  # the stored projections
+        eg, eu = eg + UH * (g.abs() + eg), eu + UH * (u.abs() + eu)  # the stored projections
         ds = s + act * (1 - s)  # |silu'| <= 1.1, |silu''| <= 0.5
         dg, du = we * dh * u * ds, we * dh * act
         edg = we * (edh * (u * ds).abs() + dh.abs() * (eu * ds.abs() + (u.abs() + eu) * 0.5 * eg)) + (U + 16 * U32) * dg.abs()
@@ -112,7 +114,7 @@ def experts(x, w, ids, wg, wu, wd, residual=None, dout=None):
         rows = dg @ Wg[e] + du @ Wu[e]
         erows = edg @ Wg[e].abs() + edu @ Wu[e].abs() + 2 * F * U32 * (dg.abs() @ Wg[e].abs() + du.abs() @ Wu[e].abs())
         r["dx"][0].index_add_(0, t, rows)
-        r["dx"][1].index_add_(0, t, erows + U * (rows.abs() + erows))
+        r["dx"][1].index_add_(0, t, erows + UH * (rows.abs() + erows))
         n = t.numel()
         r["dgate"][0][e], r["dgate"][1][e] = dg.T @ xe, edg.T @ xe.abs() + n * U32 * (dg.abs().T @ xe.abs())
         r["dup"][0][e], r["dup"][1][e] = du.T @ xe, edu.T @ xe.abs() + n * U32 * (du.abs().T @ xe.abs())
