@@ -415,13 +415,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       const size_t row0 = t.row0 + q * 32;
       const int rows = min(32, t.end - (t.row0 + q * 32));
       uint4 vg[4], vu[4];
-      float kg = 0.f, ku = 0.f;  // this lane's row's factors of the columns under way
+      uint64_t all_g = 0, all_u = 0;  // this lane's row's factors of this warp's four chunks
+      if (MODE == DHID && t.row0 + row < t.end) {
+        const size_t at = (size_t)(t.row0 + row) * p.sld + t.n0 / 32 + chunk0;
+        all_g = *reinterpret_cast<const uint64_t*>(p.s0 + at);
+        all_u = *reinterpret_cast<const uint64_t*>(p.s1 + at);
+      }
       auto fetch = [&](int c) {
-        if (t.row0 + row < t.end && t.n0 + c * 32 < p.N) {
-          const size_t at = (size_t)(t.row0 + row) * p.sld + t.n0 / 32 + c;
-          kg = __bfloat162float(p.s0[at]);
-          ku = __bfloat162float(p.s1[at]);
-        }
         const int col = t.n0 + c * 32 + c4 * 8;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -442,6 +442,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           const bool live = t.row0 + row < t.end;
           const size_t grow = t.row0 + row;
           if constexpr (MODE == GATE_UP) {
+            uint64_t all_g = 0, all_u = 0;  // the tile's four factors of this row
 #pragma unroll 1
             for (int c = 0; c < BN / 64; ++c) {
               const int col = t.n0 + c * 32;
@@ -454,10 +455,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
               if (p.out0) {
                 kg = kb::moe::block_factor(vg, back_g);
                 ku = kb::moe::block_factor(vu, back_u);
-                if (live) {
-                  p.s0[grow * p.sld + col / 32] = __float2bfloat16(back_g);
-                  p.s1[grow * p.sld + col / 32] = __float2bfloat16(back_u);
-                }
+                all_g |= (uint64_t)(__float_as_uint(back_g) >> 16) << 16 * c;
+                all_u |= (uint64_t)(__float_as_uint(back_u) >> 16) << 16 * c;
               }
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -477,6 +476,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                 }
               }
             }
+            if (live && p.out0) {
+              *reinterpret_cast<uint64_t*>(p.s0 + grow * p.sld + t.n0 / 32) = all_g;
+              *reinterpret_cast<uint64_t*>(p.s1 + grow * p.sld + t.n0 / 32) = all_u;
+            }
           } else if constexpr (MODE == DHID) {
             float dot = 0.f;
 #pragma unroll 1
@@ -489,7 +492,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                 *reinterpret_cast<uint4*>(su + staged(r, c4)) = vu[i];
               }
               __syncwarp();
-              const float fg = kg, fu = ku;
+              const float fg = __uint_as_float((uint32_t)(all_g >> 16 * (c - chunk0)) << 16), fu = __uint_as_float((uint32_t)(all_u >> 16 * (c - chunk0)) << 16);
+              const float w_u = w * fu;
+              float part_dot = 0.f;
               if (c + 1 < chunk0 + CHUNKS && t.n0 + (c + 1) * 32 < p.N) fetch(c + 1);  // under way during the arithmetic
               uint32_t v[32];
               tmem_ld_32x32b_x32(t_row + c * 32, v);
@@ -500,17 +505,18 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                 uint4* pu = reinterpret_cast<uint4*>(su + staged(lane, i));
                 float g[8], u[8], dg[8], du[8];
                 kb::moe::unpack_block8(*pg, fg, g);
-                kb::moe::unpack_block8(*pu, fu, u);
+                kb::moe::unpack_block8(*pu, 1.f, u);  // without its factor, which the sums and w_u carry
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
                   const float d = __uint_as_float(v[i * 8 + x]), s = sigmoid(g[x]), act = g[x] * s, da = d * act;
-                  dot = fmaf(da, u[x], dot);
-                  dg[x] = w * (d * u[x]) * fmaf(act, 1.f - s, s);
+                  part_dot = fmaf(da, u[x], part_dot);
+                  dg[x] = w_u * (d * u[x]) * fmaf(act, 1.f - s, s);
                   du[x] = w * da;
                 }
                 *pg = pack8(dg);
                 *pu = pack8(du);
               }
+              dot = fmaf(part_dot, fu, dot);
               __syncwarp();
               const int col = t.n0 + c * 32 + c4 * 8;
 #pragma unroll
@@ -525,6 +531,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             }
             if (live) p.part[(grow * p.num_n + t.n0 / BN) * (C::EPI / 4) + ((warp - 2) >> 2)] = dot;
           } else {
+            uint64_t low = 0, high = 0;  // the tile's eight factors of this row
 #pragma unroll 1
             for (int c = 0; c < BN / 32; ++c) {
               const int col = t.n0 + c * 32;
@@ -534,7 +541,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
               tmem_ld_wait();
               float back;
               const float k = kb::moe::block_factor(v, back);
-              if (live) p.s0[grow * p.sld + col / 32] = __float2bfloat16(back);
+              (c < 4 ? low : high) |= (uint64_t)(__float_as_uint(back) >> 16) << 16 * (c & 3);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 float f[8];
@@ -543,6 +550,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                 if (live && col + i * 8 < p.N) *reinterpret_cast<uint4*>(p.out0 + grow * p.ld0 + col + i * 8) = kb::moe::pack_block8(f, k);
               }
             }
+            if (live)
+              *reinterpret_cast<uint4*>(p.s0 + grow * p.sld + t.n0 / 32) = make_uint4((uint32_t)low, (uint32_t)(low >> 32), (uint32_t)high, (uint32_t)(high >> 32));
           }
         }
       } else {
@@ -704,7 +713,7 @@ extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, 
   p.out1 = static_cast<__nv_bfloat16*>(u);
   p.out2 = static_cast<__nv_bfloat16*>(h);
   p.ld0 = F;
-  p.sld = cdiv(F, 32);
+  p.sld = kb::moe::factor_pitch(F);
   if (g) {
     p.s0 = p.out0 + (size_t)R * F;  // the factors lie behind the values
     p.s1 = p.out1 + (size_t)R * F;
@@ -719,7 +728,7 @@ extern "C" int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, 
   p.out0 = static_cast<__nv_bfloat16*>(y);
   p.out1 = p.out2 = nullptr;
   p.ld0 = D;
-  p.sld = cdiv(D, 32);
+  p.sld = kb::moe::factor_pitch(D);
   p.s0 = p.out0 + (size_t)R * D;
   KB_TRY(launch<DOWN>(pair, a, a, b, b, p, d.dev, d.sms, st));
   return kb::moe::launch_combine(y, slots, res, ldr, out, nullptr, 0, nullptr, 0, T, k, D, R, st);
@@ -763,7 +772,7 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
   p.u = static_cast<const __nv_bfloat16*>(u);
   p.s0 = const_cast<__nv_bfloat16*>(p.g) + (size_t)R * F;
   p.s1 = const_cast<__nv_bfloat16*>(p.u) + (size_t)R * F;
-  p.sld = cdiv(F, 32);
+  p.sld = kb::moe::factor_pitch(F);
   p.rw = rw;
   p.part = part;
   KB_TRY(launch<DHID>(pair, a, a, b, b, p, d.dev, d.sms, st));
@@ -793,7 +802,7 @@ extern "C" int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, co
     p.out0 = static_cast<__nv_bfloat16*>(dys);
     p.ld0 = D;
     p.s0 = p.out0 + (size_t)R * D;
-    p.sld = cdiv(D, 32);
+    p.sld = kb::moe::factor_pitch(D);
     KB_TRY(launch<DX>(pair, a, a2, b, b2, p, d.dev, d.sms, st));
   }
   if (dx || dw) KB_TRY(kb::moe::launch_combine(dys, slots, nullptr, 0, dx, part, n_part, dw, w_f32, T, k, D, R, st));

@@ -220,7 +220,8 @@ int kb_moe_plan(const void* ids, int ids64, int n, int E, int R, int* counts, in
 // out = res + the experts' products, with the arrays of a plan (with `pair` two CTAs share a tile, of its pairs) or, where ids is
 // given, grouping them first into these arrays (counts and hist are not read otherwise); the weights [E, F, D], [E, F, D], [E, D, F]
 // (pitch, distance of the experts); scratch: xs [R,D], rw [R], h [R,F], y (may be xs); g, u (both or neither) keep the projections for the
-// backward pass.  y, g, u are fp16 blocks: [R, cols] and behind them a bf16 factor for every 32 columns, [R, ceil(cols / 32)].
+// backward pass.  y, g, u are fp16 blocks: [R, cols] and behind them a bf16 factor for every 32 columns, [R, ceil(cols / 32) up to
+// a multiple of 8].
 int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, int w_f32, const void* ids, int ids64, int* counts, int* hist, int* offsets,
                        int* slots, int* rows, int* tiles, int* pairs, int pair, const void* wg, long ldg, long sg, const void* wu, long ldu,
                        long su, const void* wd, long ldd, long sd, const void* res, long ldr, void* out, void* xs, float* rw, void* g, void* u,

@@ -33,8 +33,10 @@ cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, size_
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// fp16 blocks: 32 columns of a row share a power of two, kept as bf16 behind the [R, cols] values ([R, ceil(cols / 32)]),
-// that brings the largest of them to 2^14..2^15: 11 bits for everything down to 2^-28 of it.
+// fp16 blocks: 32 columns of a row share a power of two that brings the largest of them to 2^14..2^15: 11 bits for everything
+// down to 2^-28 of it.  Its inverse is kept as bf16 behind the [R, cols] values, [R, factor_pitch(cols)], so that the eight
+// of a 256-column tile are one 16-byte access.
+__host__ __device__ __forceinline__ int factor_pitch(int cols) { return ((cols + 31) / 32 + 7) & ~7; }
 // The factor before rounding, from the 32 fp32 accumulators; `back`: its inverse.  An infinity or a NaN stays one.
 __device__ __forceinline__ float block_factor(const uint32_t (&v)[32], float& back) {
   uint32_t m = 0;

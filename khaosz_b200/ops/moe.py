@@ -358,8 +358,8 @@ class _Space:
 
 
 def _blocks_bytes(rows: int, cols: int) -> int:
-    """``[rows, cols]`` in fp16, and behind it a bf16 factor for every 32 columns of a row."""
-    return 2 * rows * (cols + -(-cols // 32))
+    """``[rows, cols]`` in fp16, and behind it a bf16 factor for every 32 columns of a row, in multiples of eight."""
+    return 2 * rows * (cols + _round_up(-(-cols // 32), 8))
 
 
 _PLAN = ("offsets", "slots", "rows", "tiles", "pairs")
