@@ -320,7 +320,7 @@ def _where(w: Tensor) -> Tuple[int, int, int]:
 def _stacked(group: Sequence[Tensor]) -> Tensor:
     """One ``[E, rows, cols]`` tensor of a group: itself, a view over equally spaced experts, or a copy."""
     if len(group) == 1 and group[0].dim() == 3:
-        return _kernel_view(group[0].detach())
+        return _kernel_view(group[0])
     view = _uniform(group)
     return _kernel_view(view if view is not None else torch.stack([w.detach() for w in group]))
 
@@ -515,7 +515,14 @@ def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up
     if residual is not None and residual.shape != shape:
         raise ValueError(f"moe_experts: residual {tuple(residual.shape)} has not the shape of x {tuple(shape)}")
     wide = groups[0] + groups[1] + groups[2] + ((x,) if residual is None else (x, residual))   # all but the routing weights
-    if experts.device != x.device or weights.device != x.device or any(t.device != x.device for t in wide):
+    device, bf16, plain = x.device, torch.bfloat16, False
+    elsewhere = experts.device != device or weights.device != device
+    train = weights.requires_grad
+    for t in wide:
+        elsewhere = elsewhere or t.device != device
+        plain = plain or t.dtype != bf16
+        train = train or t.requires_grad
+    if elsewhere:
         raise ValueError("moe_experts: all tensors must be on one device")
     if plan is not None and (plan.slots.shape != ids_shape or plan.counts.numel() != E or plan.rows.device != x.device
                              or plan.rows.numel() != rows_bound(experts.numel(), E)):
@@ -524,11 +531,9 @@ def moe_experts(x: Tensor, weights: Tensor, experts: Tensor, w_gate: Stack, w_up
     if len(shape) != 2:
         x, weights, experts = x.reshape(-1, D), weights.reshape(-1, k), experts.reshape(-1, k)
         residual = None if residual is None else residual.reshape(-1, D)
-    bf16 = torch.bfloat16
-    if (not x.is_cuda or D % 8 or F % 8 or experts.numel() == 0 or weights.dtype not in _KERNEL_DTYPES
-            or any(t.dtype != bf16 for t in wide)):
+    if plain or not x.is_cuda or D % 8 or F % 8 or experts.numel() == 0 or weights.dtype not in _KERNEL_DTYPES:
         return _experts_torch(x, weights, experts, *(g[0] if lone else g for g in groups), residual).view(shape)
-    train = torch.is_grad_enabled() and (weights.requires_grad or any(t.requires_grad for t in wide))
+    train = train and torch.is_grad_enabled()
     x, weights, residual = _rows2d(x), weights.contiguous(), None if residual is None else _rows2d(residual)
     if not train and experts.numel() <= SMALL:
         out = _experts_small(x, weights, experts.contiguous(), residual, *(_stacked(g) for g in groups))
