@@ -464,3 +464,42 @@ def test_model_trains_captured_and_serves_captured(kind):
         assert not graphs or (ex.cuda_graphs and any(s.graph is not None for s in ex._slots.values()))
     assert outs[0] == outs[1]
     ops.raise_on_device_error()
+
+
+def test_trainer_steps_recorded_and_plain_agree():
+    """Optimizer steps of a mixture-of-experts model through an executor: the recorded micro-step (accumulated into the flat
+    gradient buffer) against plain launches.  The embedding's gradient is summed by atomics, so the two runs may part by
+    roundings; a bf16 loss of the same weights agrees to a few steps."""
+    from khaosz_b200 import AutoRegressiveLM, AutoRegressiveLMConfig
+    from khaosz_b200.parallel import ExecutorFactory
+    from khaosz_b200.trainer import FusedAdamW, StrategyFactory
+
+    def run(cuda_graph):
+        torch.manual_seed(0)
+        cfg = AutoRegressiveLMConfig(vocab_size=512, dim=256, n_layers=2, norm_eps=1e-5, dim_ffn=136, tie_weight=True, max_len=128, rope_theta=1e4, n_heads=2,
+                                     n_kv_heads=1, ffn_type="moe", n_routed_experts=8, n_shared_experts=1, n_activated_experts=2, topk_method="sigmoid",
+                                     router_bias=True)
+        model = AutoRegressiveLM(cfg).to(device="cuda", dtype=torch.bfloat16)
+        ex = ExecutorFactory.create("none", grad_accum_steps=2, cuda_graph=cuda_graph)
+        opt = FusedAdamW(model.parameters(), lr=1e-3, betas=(0.9, 0.95), weight_decay=0.01)
+        model, opt, _, _ = ex.prepare(model, opt, None, None)
+        strategy = StrategyFactory.create("seq", model, "cuda", label_smoothing=0.0)
+        losses = []
+        for step in range(4):
+            for micro in range(2):
+                g = _gen(10 * step + micro)
+                ids = torch.randint(0, 512, (2, 65), device="cuda", generator=g)
+                with ex.accumulate(model):
+                    losses.append(float(ex.micro_step(strategy, {"input_ids": ids[:, :-1], "target_ids": ids[:, 1:]})))
+                    if ex.sync_gradients:
+                        opt.fused_clip(1.0)
+                        opt.step()
+                        opt.zero_grad()
+        recorded = cuda_graph and any("graph" in e for e in ex._graphed.entries.values())
+        return losses, recorded
+
+    plain, _ = run(False)
+    graphed, recorded = run(True)
+    assert recorded
+    assert all(abs(a - b) <= 2.0 ** -6 * abs(a) for a, b in zip(plain, graphed)), (plain, graphed)
+    ops.raise_on_device_error()
