@@ -89,7 +89,7 @@ def _declare(lib):
         "kb_moe_plan": ([P, I, I, I, I, P, P, P, P, P, P, P, P], I),
         "kb_moe_experts_fwd": ([P, L, P, I, P, I, P, P, P, P, P, P, P, I, P, L, L, P, L, L, P, L, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, P], I),
         "kb_moe_experts_small": ([P, L, P, I, P, I, P, L, L, P, L, L, P, L, L, P, L, P, P, I, I, I, I, I, P], I),
-        "kb_moe_experts_bwd": ([P, L, P, P, P, P, P, P, P, P, P, I, P, L, L, P, L, L, P, L, L, P, P, P, P, P, P, P, I, P, L, L, P, L, L, P, L, L,
+        "kb_moe_experts_bwd": ([P, L, P, P, P, P, P, P, P, P, P, P, I, P, L, L, P, L, L, P, L, L, P, P, P, P, P, P, P, I, P, L, L, P, L, L, P, L, L,
                                 I, I, I, I, I, I, I, P], I),
         "kb_rmsnorm_bwd_static": ([P, P, P, P, P, P, P, I, I, P], I),
     }

@@ -230,10 +230,10 @@ int kb_moe_experts_fwd(const void* x, long ldx, const void* weights, int w_f32, 
 int kb_moe_experts_small(const void* x, long ldx, const void* weights, int w_f32, const void* ids, int ids64, const void* wg, long ldg, long sg,
                          const void* wu, long ldu, long su, const void* wd, long ldd, long sd, const void* res, long ldr, void* out, float* h,
                          int T, int k, int D, int F, int E, void* stream);
-// Backward pass (tiles: the plan's tiles, or its pairs with `pair`): dx [T,D], dw [T,k] and the weights' gradients, each optional (dwg and dwu together); accumulate: the weights' gradients are
+// Backward pass: dx [T,D], dw [T,k] and the weights' gradients, each optional (dwg and dwu together); accumulate: the weights' gradients are
 // added to what is there.  Scratch: dys (fp16 blocks of D columns), dg, du [R,F], part [R, 2 ceil(F / 256)], order [E].
 int kb_moe_experts_bwd(const void* dout, long ldo, const void* xs, const float* rw, const void* g, const void* u, const void* h,
-                       const int* offsets, const int* slots, const int* rows, const int* tiles, int pair, const void* wg, long ldg, long sg, const void* wu,
+                       const int* offsets, const int* slots, const int* rows, const int* tiles, const int* pairs, int pair, const void* wg, long ldg, long sg, const void* wu,
                        long ldu, long su, const void* wd, long ldd, long sd, void* dys, void* dg, void* du, float* part, int* order, void* dx, void* dw,
                        int w_f32, void* dwg, long ldwg, long sdwg, void* dwu, long ldwu, long sdwu, void* dwd, long ldwd, long sdwd,
                        int accumulate, int T, int k, int D, int F, int E, int R, void* stream);

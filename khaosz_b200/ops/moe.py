@@ -335,10 +335,10 @@ def _grad_view(group: Sequence[Tensor]) -> Optional[Tensor]:
 
 
 def _use_pairs(n: int, E: int) -> bool:
-    """Whether two CTAs share a tile of 256 rows of the grouped products.  Pairs read a third less from L2, but half of a pair's
-    tile is wasted on an expert's last 128 rows.  Measured on a B200 (D 2048, F 1408, 16 experts, forward and training step): at
-    768 rows per expert 226 and 826 us alone against 238 and 872 us in pairs, at 2048 rows the products take 1548 us alone and
-    1427 us in pairs."""
+    """Whether two CTAs share a tile of 256 rows of the products that have both forms.  Pairs read a third less from L2, but half
+    of a pair's tile is wasted on an expert's last 128 rows.  Measured on a B200 (D 2048, F 1408, 16 experts, forward and training
+    step): at 768 rows per expert 226 and 826 us alone against 238 and 872 us in pairs; at 2048 rows the three products that
+    have both forms take 797 us alone and 753 us in pairs."""
     return n >= 1024 * E
 
 
@@ -416,7 +416,6 @@ class _ExpertsFn(torch.autograd.Function):
         at = ctx.space.addresses(buf)
         if plan:
             at.update((name, t.data_ptr()) for name, t in zip(MoEPlan._fields, plan))
-        pair = _use_pairs(T * k, E)
         dout = _rows2d(dout)
         dev = dout.device
         sp = _Space(dev, dict(dys=_blocks_bytes(R, D), dg=2 * R * F, du=2 * R * F, part=4 * R * 2 * -(-F // 256), order=4 * E))
@@ -432,7 +431,7 @@ class _ExpertsFn(torch.autograd.Function):
             grads = [torch.empty(w.shape, dtype=w.dtype, device=dev) if wanted else None for w, wanted in ((wg, gate_up), (wu, gate_up), (wd, down))]
         where = [v for g in grads for v in (_where(g) if g is not None else (None, 0, 0))]
         _call(dout, "kb_moe_experts_bwd", dout.data_ptr(), _pitch(dout), at["xs"], at["rw"], at["g"], at["u"], at["h"],
-              at["offsets"], at["slots"], at["rows"], at["pairs" if pair else "tiles"], pair, *_where(wg), *_where(wu), *_where(wd), *scratch.values(),
+              *(at[name] for name in _PLAN), _use_pairs(T * k, E), *_where(wg), *_where(wu), *_where(wd), *scratch.values(),
               _p(dx), _p(dw), w_dtype == torch.float32, *where, into, T, k, D, F, E, R)
         _lib.add_launches(1 + (grads[2] is not None) + (dx is not None) + (dx is not None or dw is not None) + (grads[0] is not None))
         out = []
