@@ -784,6 +784,7 @@ extern "C" int kb_moe_route_bwd(const void* z, int z_f32, long ldz, const float*
   RouteParams p{z, bias, nullptr, const_cast<long long*>(ids), ldz, T, E, k, sigmoid, renorm, 1, 1, 1, w_f32, scale};
   if (const int rc = route_check(p)) return rc;
   if (T == 0) return KB_STATUS_OK;
+  if (reinterpret_cast<uintptr_t>(dz) & 15) return KB_STATUS_BAD_ARG;  // rows are cleared in 16-byte pieces
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (z_f32) route_bwd<float>(p, dw, dz, st);
   else route_bwd<__nv_bfloat16>(p, dw, dz, st);
